@@ -46,6 +46,17 @@ class GgufTensorInfo(ctypes.Structure):
                 ("nbytes", ctypes.c_uint64), ("data", ctypes.c_void_p)]
 
 
+class KvPages(ctypes.Structure):
+    """engine_kv_pages_t (include/engine_b200.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("length", ctypes.c_void_p), ("ref", ctypes.c_void_p),
+                ("n_layers", ctypes.c_int64), ("n_pages", ctypes.c_int64),
+                ("n_kv_heads", ctypes.c_int64), ("page_size", ctypes.c_int64),
+                ("head_dim", ctypes.c_int64), ("n_slots", ctypes.c_int64),
+                ("max_pages", ctypes.c_int64), ("type", ctypes.c_int32)]
+
+
 # name -> (argtypes) ; every entry returns int status
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -84,6 +95,14 @@ EXPORTS: dict[str, list] = {
                                         _p],
     "engine_cuda_rmsnorm_linear_kv_f16": [_p, _p, _p, _p, _p, _i64, _i64, _f, _p, _p, _i64, _i64,
                                           _i64, _i64, _i64, _p],
+    "engine_cuda_kv_pages_extend": [_p, _p, _p, _p, _i64, _p],
+    "engine_cuda_kv_pages_fork": [_p, _p, _p, _p, _i64, _p],
+    "engine_cuda_kv_pages_free": [_p, _p, _i64, _p],
+    "engine_cuda_kv_pages_compact": [_p, _p, _p],
+    "engine_cuda_kv_pages_write": [_p, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _p],
+    "engine_cuda_attention_paged_decode": [_p, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _f, _p],
+    "engine_cuda_attention_paged_prefill": [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64,
+                                            _f, ctypes.c_int, _p],
     "engine_gguf_open": [ctypes.c_char_p, _P(ctypes.c_void_p)],
     "engine_gguf_close": [_p],
     "engine_gguf_version": [_p, _P(ctypes.c_int32), _P(ctypes.c_uint64)],

@@ -7,7 +7,9 @@ raises :class:`EngineError` when the library rejects the call.
 """
 from __future__ import annotations
 
-from . import _check, lib
+import ctypes
+
+from . import KvPages, _check, lib
 
 
 def _s(stream) -> int | None:
@@ -199,3 +201,47 @@ def tp_allreduce_f16(comm, partial, residual, y, n, stream=0):
 def tp_linear_allreduce_f16(comm, X, W, residual, Y, M, N, K, stream=0):
     _check(lib().engine_tp_linear_allreduce_f16(comm, X, W, residual, Y, M, N, K, _s(stream)))
 
+
+# Paged 8-bit KV cache (engine_b200.h): no counterpart in kernels.hpp.  `kv` is a
+# KvPages structure (or its address); ops.PagedKV builds one from torch tensors.
+KV_I8 = 1
+KV_E4M3 = 2
+KV_MAX_SLOTS = 2048
+
+
+def _kv(kv):
+    return ctypes.addressof(kv) if isinstance(kv, KvPages) else kv
+
+
+def kv_pages_extend(kv, slots, n_new, status, n, stream=0):
+    _check(lib().engine_cuda_kv_pages_extend(_kv(kv), slots, n_new, status, n, _s(stream)))
+
+
+def kv_pages_fork(kv, parents, children, status, n, stream=0):
+    _check(lib().engine_cuda_kv_pages_fork(_kv(kv), parents, children, status, n, _s(stream)))
+
+
+def kv_pages_free(kv, slots, n, stream=0):
+    _check(lib().engine_cuda_kv_pages_free(_kv(kv), slots, n, _s(stream)))
+
+
+def kv_pages_compact(kv, remap=0, stream=0):
+    _check(lib().engine_cuda_kv_pages_compact(_kv(kv), remap, _s(stream)))
+
+
+def kv_pages_write(kv, layer, k_new, v_new, row_pitch, slots, cu_new, n_seq, n_tokens, stream=0):
+    _check(lib().engine_cuda_kv_pages_write(_kv(kv), layer, k_new, v_new, row_pitch, slots, cu_new,
+                                            n_seq, n_tokens, _s(stream)))
+
+
+def attention_paged_decode(kv, layer, q, q_pitch, slots, out, out_lse, n_seq, n_heads, scale,
+                           stream=0):
+    _check(lib().engine_cuda_attention_paged_decode(_kv(kv), layer, q, q_pitch, slots, out, out_lse,
+                                                    n_seq, n_heads, scale, _s(stream)))
+
+
+def attention_paged_prefill(kv, layer, q, q_pitch, slots, cu_q, out, out_lse, n_seq, n_tokens,
+                            n_heads, scale, is_causal=True, stream=0):
+    _check(lib().engine_cuda_attention_paged_prefill(_kv(kv), layer, q, q_pitch, slots, cu_q, out,
+                                                     out_lse, n_seq, n_tokens, n_heads, scale,
+                                                     1 if is_causal else 0, _s(stream)))

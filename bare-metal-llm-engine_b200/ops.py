@@ -6,8 +6,11 @@ stated dtype (checked here, loudly); outputs are allocated when not given.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
+from . import KvPages as _KvPages
 from . import cuda as _c
 
 
@@ -255,6 +258,193 @@ def attention_decode_cached(q, k_cache, v_cache, kv_len: int, scale=None, out=No
     _c.attention_decode(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), kv_len,
                         H, H_kv, d, max_len * d, scale, 0, _stream())
     return o
+
+
+class PagedKV:
+    """An 8-bit paged KV cache (engine_kv_pages_t): the tensors, and the handle that
+    the kv_pages_* and attention_paged_* calls take.
+
+    k, v              [n_layers, n_pages, H_kv, page, d] int8 or float8_e4m3fn codes
+    k_scale, v_scale  [n_layers, n_pages, H_kv] float32; value = scale * code
+    table             [n_slots, max_pages] int32, a slot's pages by position (-1: none)
+    length            [n_slots] int32, tokens of each slot
+    ref               [n_pages] int32, slots that use a page (0: free)
+
+    The tensors stay the caller's and may be read at any time; the kernels keep
+    table, length and ref, so they are not to be replaced by others afterwards."""
+
+    def __init__(self, k, v, k_scale, v_scale, table, length, ref):
+        if k.dtype not in (torch.int8, torch.float8_e4m3fn):
+            raise TypeError(f"k must be int8 or float8_e4m3fn, got {k.dtype}")
+        if k.dim() != 5 or v.shape != k.shape:
+            raise ValueError("k and v must be [n_layers, n_pages, H_kv, page, d], of one shape")
+        n_layers, n_pages, hk, page, d = k.shape
+        for t, dt, shape, n in ((k, k.dtype, k.shape, "k"), (v, k.dtype, k.shape, "v"),
+                                (k_scale, torch.float32, k.shape[:3], "k_scale"),
+                                (v_scale, torch.float32, k.shape[:3], "v_scale"),
+                                (table, torch.int32, None, "table"),
+                                (length, torch.int32, table.shape[:1], "length"),
+                                (ref, torch.int32, k.shape[1:2], "ref")):
+            _req(t, dt, n)
+            if shape is not None and t.shape != shape:
+                raise ValueError(f"{n} must be {tuple(shape)}, got {tuple(t.shape)}")
+            if t.device != k.device:
+                raise ValueError(f"{n} must be on {k.device}")
+        if table.dim() != 2:
+            raise ValueError("table must be [n_slots, max_pages]")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.table, self.length, self.ref = table, length, ref
+        self.n_slots, self.max_pages = table.shape
+        self.n_kv_heads, self.head_dim, self.n_pages = hk, d, n_pages
+        self.device_index = k.device.index
+        self.desc = _KvPages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                             table.data_ptr(), length.data_ptr(), ref.data_ptr(), n_layers, n_pages,
+                             hk, page, d, self.n_slots, self.max_pages,
+                             _c.KV_I8 if k.dtype == torch.int8 else _c.KV_E4M3)
+        self.handle = ctypes.addressof(self.desc)
+
+    @classmethod
+    def empty(cls, n_layers, n_pages, n_kv_heads, page_size, head_dim, n_slots, max_pages,
+              dtype=torch.int8, device="cuda"):
+        """A new cache without sequences."""
+        shape = (n_layers, n_pages, n_kv_heads, page_size, head_dim)
+        z = dict(device=device, dtype=torch.int32)
+        return cls(torch.empty(shape, device=device, dtype=dtype),
+                   torch.empty(shape, device=device, dtype=dtype),
+                   torch.zeros(shape[:3], device=device), torch.zeros(shape[:3], device=device),
+                   torch.full((n_slots, max_pages), -1, **z), torch.zeros(n_slots, **z),
+                   torch.zeros(n_pages, **z))
+
+
+def _kv_req(kv, *named):
+    """The calls' checks: the cache on the current device, int32 arguments beside it."""
+    if kv.device_index != torch.cuda.current_device():
+        raise ValueError(f"the cache is on cuda:{kv.device_index}, which is not the current device")
+    for t, n in named:
+        _req(t, torch.int32, n)
+        if t.device.index != kv.device_index:
+            raise ValueError(f"{n} must be on the cache's device")
+
+
+def _kv_slots(kv, slots, n):
+    """Entries of a call over `slots` (None: slots 0 .. n - 1)."""
+    if slots is not None and slots.numel() != n:
+        raise ValueError(f"slots must have {n} entries, got {slots.numel()}")
+    return _ptr(slots)
+
+
+def kv_pages_extend(kv, slots, n_new):
+    """Adds n_new[i] tokens to slot slots[i] (int32 tensors; slots None: 0, 1, ...),
+    taking the pages they need, lowest free id first.  Returns status [1] int32:
+    0, or the number of missing pages, or -1 for a bad argument; unless 0, nothing
+    changed.  Nothing is synchronised: read the status when it is wanted."""
+    _kv_req(kv, (n_new, "n_new"), *(() if slots is None else ((slots, "slots"),)))
+    status = torch.empty(1, device=n_new.device, dtype=torch.int32)
+    n = n_new.numel()
+    _c.kv_pages_extend(kv.handle, _kv_slots(kv, slots, n), n_new.data_ptr(), status.data_ptr(), n,
+                       _stream())
+    return status
+
+
+def kv_pages_fork(kv, parents, children):
+    """Makes the empty slots children[i] copies of parents[i]: full pages shared, the
+    partly filled one copied in all layers.  Returns status as kv_pages_extend."""
+    _kv_req(kv, (parents, "parents"), (children, "children"))
+    if parents.numel() != children.numel():
+        raise ValueError("parents and children must have as many entries")
+    status = torch.empty(1, device=parents.device, dtype=torch.int32)
+    _c.kv_pages_fork(kv.handle, parents.data_ptr(), children.data_ptr(), status.data_ptr(),
+                     parents.numel(), _stream())
+    return status
+
+
+def kv_pages_free(kv, slots):
+    """Empties the slots; pages without a user left are free again."""
+    _kv_req(kv, (slots, "slots"))
+    _c.kv_pages_free(kv.handle, slots.data_ptr(), slots.numel(), _stream())
+
+
+def kv_pages_compact(kv):
+    """Moves the pages in use to the lowest ids, in all layers; tables and ref follow.
+    Returns remap [n_pages] int32: the new id of each page, -1 if it was free."""
+    _kv_req(kv)
+    remap = torch.empty(kv.n_pages, device=kv.ref.device, dtype=torch.int32)
+    _c.kv_pages_compact(kv.handle, remap.data_ptr(), _stream())
+    return remap
+
+
+def kv_pages_write(kv, layer: int, k_rows, v_rows, slots=None, cu_new=None):
+    """Stores K / V rows [n_tokens, H_kv * d] (FP16, rows may be strided views, e.g. the
+    columns of a fused Q/K/V projection) as the LAST positions of the slots: rows
+    [cu_new[i], cu_new[i+1]) of slot slots[i], or one row each where cu_new is None.
+    Call kv_pages_extend first: it counts them."""
+    _kv_req(kv, *(() if slots is None else ((slots, "slots"),)),
+            *(() if cu_new is None else ((cu_new, "cu_new"),)))
+    for t, n in ((k_rows, "k_rows"), (v_rows, "v_rows")):
+        if t.dtype != torch.float16 or not t.is_cuda:
+            raise TypeError(f"{n} must be a CUDA float16 tensor")
+        if t.dim() != 2 or t.shape[1] != kv.n_kv_heads * kv.head_dim:
+            raise ValueError(f"{n} must be [n_tokens, H_kv * d]")
+        if t.device.index != kv.device_index:
+            raise ValueError(f"{n} must be on the cache's device")
+    if k_rows.shape != v_rows.shape or k_rows.stride() != v_rows.stride() or k_rows.stride(1) != 1:
+        raise ValueError("k_rows / v_rows: rows must be contiguous, as many, and share one pitch")
+    n_tokens = k_rows.shape[0]
+    n_seq = n_tokens if cu_new is None else cu_new.numel() - 1
+    pitch = k_rows.stride(0) if n_tokens > 1 else max(k_rows.stride(0), k_rows.shape[1])
+    _c.kv_pages_write(kv.handle, layer, k_rows.data_ptr(), v_rows.data_ptr(), pitch,
+                      _kv_slots(kv, slots, n_seq), _ptr(cu_new), n_seq, n_tokens, _stream())
+
+
+def _paged_q(kv, q, out):
+    """Checks q [n, H, d] (heads contiguous, rows may be strided) and out; (pitch, out)."""
+    if q.dtype != torch.float16 or not q.is_cuda:
+        raise TypeError("q must be a CUDA float16 tensor")
+    if q.dim() != 3 or q.shape[2] != kv.head_dim:
+        raise ValueError("q must be [n, H, d]")
+    if q.device.index != kv.device_index:
+        raise ValueError("q must be on the cache's device")
+    n, H, d = q.shape
+    if q.stride(2) != 1 or (H > 1 and q.stride(1) != d):
+        raise ValueError("q: the heads of a row must be contiguous")
+    if out is None:
+        out = torch.empty(q.shape, device=q.device, dtype=torch.float16)
+    else:
+        _req(out, torch.float16, "out")
+        if out.shape != q.shape:
+            raise ValueError("out must have q's shape")
+    return (q.stride(0) if n > 1 else max(q.stride(0), H * d)), out
+
+
+def attention_paged_decode(kv, layer: int, q, slots=None, scale=None, out=None,
+                           want_lse: bool = False):
+    """out [B, H, d] of one query row per sequence, q [B, H, d], over all positions of
+    the slots (None: slots 0 .. B - 1); with want_lse also lse [B, H] (FP32)."""
+    _kv_req(kv, *(() if slots is None else ((slots, "slots"),)))
+    pitch, o = _paged_q(kv, q, out)
+    B, H, d = q.shape
+    lse = torch.empty(B, H, device=q.device, dtype=torch.float32) if want_lse else None
+    _c.attention_paged_decode(kv.handle, layer, q.data_ptr(), pitch, _kv_slots(kv, slots, B),
+                              o.data_ptr(), _ptr(lse), B, H, d ** -0.5 if scale is None else scale,
+                              _stream())
+    return (o, lse) if want_lse else o
+
+
+def attention_paged_prefill(kv, layer: int, q, slots, cu_q, scale=None, out=None,
+                            is_causal: bool = True, want_lse: bool = False):
+    """out [T, H, d] of the query rows [cu_q[i], cu_q[i+1]) of q [T, H, d], the LAST
+    positions of slot slots[i] (None: slot i), over the slot's positions up to their
+    own (all of them unless is_causal).  Rows past cu_q[-1] are left as they were in
+    `out`.  With want_lse also lse [T, H] (FP32)."""
+    _kv_req(kv, (cu_q, "cu_q"), *(() if slots is None else ((slots, "slots"),)))
+    pitch, o = _paged_q(kv, q, out)
+    T, H, d = q.shape
+    n_seq = cu_q.numel() - 1
+    lse = torch.empty(T, H, device=q.device, dtype=torch.float32) if want_lse else None
+    _c.attention_paged_prefill(kv.handle, layer, q.data_ptr(), pitch, _kv_slots(kv, slots, n_seq),
+                               cu_q.data_ptr(), o.data_ptr(), _ptr(lse), n_seq, T, H,
+                               d ** -0.5 if scale is None else scale, is_causal, _stream())
+    return (o, lse) if want_lse else o
 
 
 def swiglu(gate, up, out=None):

@@ -379,6 +379,126 @@ ENGINE_B200_API int engine_cuda_rmsnorm_linear_kv_f16(
     int64_t head_dim, int64_t max_len, int64_t pos, engine_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Paged KV cache held in 8 bits.  No counterpart in the reference, whose caches
+ * are FP16, contiguous and of one length (kernels.hpp:184); this is the cache of
+ * a serving batch: sequences of any lengths, sharing the pages of common
+ * prefixes, at half the bytes.
+ *
+ * A page holds page_size tokens of all KV heads of a layer; a (page, head) has
+ * one FP32 scale for K and one for V, and the value of a code is scale * code.
+ * Page ids are common to all layers.  Row s of `table` lists the pages of slot
+ * s in the order of its positions; `length` counts its tokens; `ref` counts the
+ * slots that use a page (0 = free).  Before the first use: table all -1, length
+ * and ref all 0.  A page that is only partly filled has one user.
+ *
+ * All of it is device memory that the kernels read, so the calls need no host
+ * synchronisation and can be captured; calls that use one cache are ordered by
+ * the caller (one stream, or events).  Entries that are out of range -- a slot
+ * outside [0, n_slots), a length beyond the row, a page id outside [0, n_pages)
+ * -- set error bit 2 (engine_device_status) and are left out.
+ *
+ * `slots` (device, n entries; may be null: slot i for entry i) names the slots
+ * that a call works on.  k and v are 16-byte aligned.
+ * ------------------------------------------------------------------------- */
+#define ENGINE_KV_I8 1   /* int8 codes, scale = max |x| / 127 */
+#define ENGINE_KV_E4M3 2 /* FP8 e4m3 codes, scale = max |x| / 448 */
+
+typedef struct {
+  void* k;          /* codes [n_layers][n_pages][n_kv_heads][page_size][head_dim] */
+  void* v;
+  float* k_scale;   /* [n_layers][n_pages][n_kv_heads] */
+  float* v_scale;
+  int32_t* table;   /* [n_slots][max_pages] */
+  int32_t* length;  /* [n_slots] */
+  int32_t* ref;     /* [n_pages] */
+  int64_t n_layers, n_pages, n_kv_heads;
+  int64_t page_size; /* 16, 32, 64 or 128 */
+  int64_t head_dim;  /* 64 or 128 */
+  int64_t n_slots, max_pages;
+  int32_t type;      /* ENGINE_KV_* */
+} engine_kv_pages_t;
+
+/* Most slots of one extend / fork call. */
+#define ENGINE_KV_MAX_SLOTS 2048
+
+/* length[slots[i]] += n_new[i], taking the pages that this needs from the free
+ * ones, lowest id first, in the order of i and then of position.  All or
+ * nothing: *status (device) = 0, or the number of pages that were missing, or
+ * -1 (and error bit 2) for a slot out of range or named twice, a negative n_new
+ * or a row too short; unless 0, nothing changed. */
+ENGINE_B200_API int engine_cuda_kv_pages_extend(const engine_kv_pages_t* kv, const int32_t* slots,
+                                                const int32_t* n_new, int32_t* status, int64_t n,
+                                                engine_stream_t stream);
+
+/* Slot children[i] (empty before) becomes a copy of slot parents[i]: full pages
+ * are shared, and a partly filled last page is copied, in all layers, to a free
+ * page (lowest id first, in the order of i).  A parent may occur several times;
+ * a child may not, nor be a parent.  *status as for extend (a child that is not
+ * empty: -1). */
+ENGINE_B200_API int engine_cuda_kv_pages_fork(const engine_kv_pages_t* kv, const int32_t* parents,
+                                              const int32_t* children, int32_t* status, int64_t n,
+                                              engine_stream_t stream);
+
+/* Empties the slots: their pages lose a user, their rows become -1, their
+ * lengths 0.  An empty slot, or the same slot twice, is no error. */
+ENGINE_B200_API int engine_cuda_kv_pages_free(const engine_kv_pages_t* kv, const int32_t* slots,
+                                              int64_t n, engine_stream_t stream);
+
+/* Moves the pages in use to the ids [0, number in use): the k-th free id below
+ * that takes the k-th used page at or past it, in all layers, and every row and
+ * `ref` follow.  remap[p] (n_pages entries, may be null) = the new id of page p,
+ * -1 if it was free. */
+ENGINE_B200_API int engine_cuda_kv_pages_compact(const engine_kv_pages_t* kv, int32_t* remap,
+                                                 engine_stream_t stream);
+
+/* Stores new keys and values: sequence i (slot slots[i]) has the rows
+ * [cu_new[i], cu_new[i+1]) of k_new / v_new (row r at r * row_pitch elements,
+ * [n_kv_heads][head_dim] each), which are its LAST positions (extend first, so
+ * that length counts them).  cu_new null: one row each.  cu_new[n_seq] may be
+ * below n_tokens: the rows past it are not read.
+ *   For every (page, head) with m = max |x| over the new rows in it: a page
+ * that starts with a new row gets scale m * (1/Q), Q = 127 or 448; a page with
+ * earlier rows gets max(its scale, m * (1/Q)), and where that grows, its other
+ * codes q become round(q * (old / new)).  A new row's codes are round(x * (1 / scale))
+ * (0 for scale 0).  An infinity or NaN cannot be held in 8 bits: the scale
+ * becomes NaN, so that attention to that (page, head) answers NaN.
+ *   Pages written to must have one user.  k_new, v_new 16-byte aligned, row_pitch
+ * a multiple of 8. */
+ENGINE_B200_API int engine_cuda_kv_pages_write(const engine_kv_pages_t* kv, int64_t layer,
+                                               const engine_half_t* k_new,
+                                               const engine_half_t* v_new, int64_t row_pitch,
+                                               const int32_t* slots, const int32_t* cu_new,
+                                               int64_t n_seq, int64_t n_tokens,
+                                               engine_stream_t stream);
+
+/* attention_decode (kernels.hpp:191) over the paged cache for a ragged batch:
+ * out[i][h] = softmax(scale q[i][h] K^T) V over the length[slots[i]] positions of
+ * its slot.  q row i at i * q_pitch elements, [n_heads][head_dim]; out
+ * [n_seq][n_heads][head_dim] and out_lse [n_seq][n_heads] (natural log, may be
+ * null) contiguous.  An empty slot gives zeros and -inf.  q and out 16-byte
+ * aligned, q_pitch a multiple of 8. */
+ENGINE_B200_API int engine_cuda_attention_paged_decode(const engine_kv_pages_t* kv, int64_t layer,
+                                                       const engine_half_t* q, int64_t q_pitch,
+                                                       const int32_t* slots, engine_half_t* out,
+                                                       float* out_lse, int64_t n_seq,
+                                                       int64_t n_heads, float scale,
+                                                       engine_stream_t stream);
+
+/* attention_prefill (kernels.hpp:153) over the paged cache for a ragged batch:
+ * the rows [cu_q[i], cu_q[i+1]) of q are the LAST positions of slot slots[i]
+ * (written before the call); when causal, each sees the positions up to its own,
+ * otherwise all of the slot's.  Rows that see nothing get zeros and -inf; the
+ * rows from cu_q[n_seq] to n_tokens are left as they were.  q, out, out_lse as
+ * for attention_paged_decode, with n_tokens rows. */
+ENGINE_B200_API int engine_cuda_attention_paged_prefill(const engine_kv_pages_t* kv, int64_t layer,
+                                                        const engine_half_t* q, int64_t q_pitch,
+                                                        const int32_t* slots, const int32_t* cu_q,
+                                                        engine_half_t* out, float* out_lse,
+                                                        int64_t n_seq, int64_t n_tokens,
+                                                        int64_t n_heads, float scale, int is_causal,
+                                                        engine_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * GGUF model files, memory-mapped, feeding the projections.  The engine plans a
  * GGUF-style mmap'd loader (README.md:247, Module 7; tensor.hpp:19-23: weight
  * tensors aliasing one mapped region) but has none; this is that loader's
