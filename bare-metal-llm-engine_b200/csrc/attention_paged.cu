@@ -9,7 +9,28 @@
 // what it contributes.  A page whose values are all zero has scale 0: it counts
 // with vs = 1 (its codes are zeros).
 //
-// First form: one warp per query row and head, FP32 on CUDA cores.
+// Few query rows per KV head (decode, and the verification of a few tokens): the
+// keys and values are the traffic, 2 bytes for 4 * rows FLOP, so what counts is
+// that the codes stream at HBM rate and cost few instructions each.
+//   Work split: an item is (sequence, 16 query rows, KV head); its keys are tiles of
+// 64.  All tiles of all items are laid end to end and every CTA takes an equal
+// range of them, whatever the lengths are (they are on the device; the host knows
+// none).  An item inside one range is written out at once; of one that is cut, each
+// CTA leaves (m, l, O) in a workspace, and a second kernel joins them in order.
+//   A CTA: one producer warp and four consumer warps.  The producer looks up pages
+// and scales, 32 slices of 16 keys at a time and one batch ahead, and fetches each
+// tile's K and V codes by TMA into a ring of kStages x 64 keys (rows of 128 bytes,
+// 128-byte swizzle); each consumer warp owns 16 keys of every tile.
+//   Products: mma.sync m16n8k16 with the query rows as A.  tcgen05 would want its
+// operands as FP16 in shared memory, and writing the widened codes there and back
+// costs more than the products (16 rows x 16 keys x 2 d FLOP against 16 x 2 d
+// bytes); here a lane turns the bytes that it has just loaded into B fragments in
+// registers.  The order of the contraction is free, so a lane's B elements are
+// consecutive bytes: D / 4 of one key's row for Q K^T, D / 8 of four keys' rows for
+// P V.  S comes out in the layout that P V wants as its A operand.
+
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "kernels.cuh"
@@ -18,110 +39,631 @@
 namespace b200 {
 namespace {
 
+constexpr int kPgKeys = 64;      // keys per tile
+constexpr int kPgRows = 16;      // query rows per item
+constexpr int kPgConsumers = 4;  // warps; each takes 16 keys of a tile
+constexpr int kPgThreads = (kPgConsumers + 1) * 32;
+constexpr int kPgMaxSeq = 1024;  // sequences per launch (their prefix sums sit in shared memory)
+constexpr float kPgRescale = 8.0f;
+
 struct ApParams {
   KvView c;
   const __half* q;
   int64_t q_pitch;
   const int32_t* slots;
-  const int32_t* cu;  // null: one row per sequence, all keys
+  const int32_t* cu;  // null: one row per sequence
   __half* out;
   float* lse;
-  int64_t n_seq, n_tokens;
-  int n_heads;
+  int seq0, n_seq;    // sequences [seq0, seq0 + n_seq) of the call
+  int64_t n_tokens;
+  int n_heads, group;
   int causal;
   float scale_log2;
+  float* ws_o;        // [2 * CTAs][rows][D]
+  float2* ws_ml;      // [2 * CTAs][rows]
+  int4* cut;          // [CTAs]: the item that a CTA began and did not finish
+  unsigned long long limit_ns;
 };
 
-template <int D, bool E4M3>
-__global__ void __launch_bounds__(128) attn_paged_simple_kernel(const ApParams p) {
+template <int D>
+struct PgCfg {
+  static constexpr int kTile = kPgKeys * D;  // bytes of K (or V) of a tile
+  static constexpr int kStages = D == 128 ? 4 : 6;
+  static constexpr int kOffO = kStages * 2 * kTile;
+  static constexpr int kOffConst = kOffO + kPgRows * D * 4;
+  static constexpr int kOffBar = kOffConst + kStages * 4 * 16;
+  static constexpr int kOffMl = kOffBar + 2 * kStages * 8;
+  static constexpr int kOffSeq = kOffMl + kPgConsumers * kPgRows * 8;
+  static size_t smem(int n_seq) { return kOffSeq + 12 * (static_cast<size_t>(n_seq) + 1) + 1024; }
+};
+
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+/// d += a b, m16n8k16.  With R8, rows 8..15 of a are zero and of d unused.  The whole
+/// warp has to come here together: callers put __syncwarp() behind code that the lanes'
+/// rows may branch in (a row's own branch around its sum lost parts of O).
+template <bool R8>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (R8) {
+    float x, y;
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, "
+        "{%0, %1, %9, %9};"
+        : "+f"(d[0]), "+f"(d[1]), "=f"(x), "=f"(y)
+        : "r"(a[0]), "r"(0), "r"(a[2]), "r"(b0), "r"(b1), "f"(0.0f));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+
+/// Shared-memory offset, within a tile, of the 16 bytes `c` of key `key`'s row.
+template <int D>
+__device__ __forceinline__ uint32_t pg_at(int key, int c) {
+  if constexpr (D == 128) {
+    return key * 128 + ((c ^ (key & 7)) << 4);
+  } else {  // two keys to a 128-byte row
+    const int line = key >> 1;
+    return line * 128 + (((((key & 1) << 2) | c) ^ (line & 7)) << 4);
+  }
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+
+/// Barrier of the consumer warps.  bar.sync wants whole warps: lanes that parted
+/// before it (a row's own branch, a loop's early exit) are brought together first.
+__device__ __forceinline__ void consumer_sync() {
+  __syncwarp();
+  named_barrier_sync(1, kPgConsumers * 32);
+}
+
+/// An item and the part of it that a CTA takes.
+struct PgItem {
+  int b;         // sequence, within the launch
+  int slot, len;
+  int head;      // KV head
+  int row0;      // first flat query row (token * group + head within the group)
+  int n_rows;    // flat rows of the sequence
+  int n_tok;     // its tokens
+  int64_t first; // its first token
+  int t0, t1;    // tiles
+  int begin;     // the item's first tile, counted over all items
+  int tiles;     // of the whole item
+};
+
+struct PgLists {
+  const int32_t* pre;   // tiles before each sequence
+  const int32_t* slot;
+  const int32_t* len;
+};
+
+/// The item at tile `x`, up to tile `hi`.
+__device__ __forceinline__ PgItem pg_item(const ApParams& p, const PgLists& s, int x, int hi) {
+  int lo = 0, up = p.n_seq - 1;
+  while (lo < up) {  // the last sequence that starts at or before x
+    const int mid = (lo + up + 1) >> 1;
+    if (s.pre[mid] <= x) lo = mid;
+    else up = mid - 1;
+  }
+  PgItem it;
+  it.b = lo;
+  it.slot = s.slot[lo];
+  it.len = s.len[lo];
+  it.tiles = max((it.len + kPgKeys - 1) / kPgKeys, 1);
+  const int y = x - s.pre[lo];
+  const int j = y / it.tiles;
+  it.t0 = y - j * it.tiles;
+  it.t1 = min(it.tiles, it.t0 + hi - x);
+  it.begin = x - it.t0;
+  it.head = j % p.c.heads;
+  it.row0 = j / p.c.heads * kPgRows;
+  it.n_tok = kv_rows(p.c, p.cu, p.seq0 + lo, p.n_tokens, &it.first);
+  it.n_rows = it.n_tok * p.group;
+  return it;
+}
+
+/// Row of out / lse of a flat query row of a sequence.
+__device__ __forceinline__ int64_t pg_row(const ApParams& p, int64_t first, int head, int flat) {
+  const int tok = flat / p.group;
+  return (first + tok) * p.n_heads + head * p.group + (flat - tok * p.group);
+}
+
+template <int D, bool E4M3, bool R8>
+__global__ void __launch_bounds__(kPgThreads, 3)
+    attn_paged_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                      const ApParams p) {
+  using Cfg = PgCfg<D>;
+  constexpr int ST = Cfg::kStages;
+  constexpr int NR = R8 ? 1 : 2;  // query rows per lane: g and g + 8
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  float* s_o = reinterpret_cast<float*>(smem + Cfg::kOffO);
+  float4* s_const = reinterpret_cast<float4*>(smem + Cfg::kOffConst);  // [ST][4]: of 16 keys each
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
+  uint64_t* empty = full + ST;
+  float2* s_ml = reinterpret_cast<float2*>(smem + Cfg::kOffMl);        // [warps][rows]
+  int32_t* s_pre = reinterpret_cast<int32_t*>(smem + Cfg::kOffSeq);    // [n_seq + 1]
+  int32_t* s_slot = s_pre + p.n_seq + 1;
+  int32_t* s_len = s_slot + p.n_seq + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kPgConsumers);
+    }
+    fence_barrier_init();
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+  }
   pdl_trigger();
   pdl_wait();
-  const int64_t task = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (task >= p.n_tokens * p.n_heads) return;
-  const int64_t t = task / p.n_heads;
-  const int h = static_cast<int>(task % p.n_heads);
-  int64_t b = -1, first = t;
-  int n = 1;
-  if (p.cu == nullptr) {
-    b = t;
+  // Tiles of each sequence, then their sums.
+  for (int b = threadIdx.x; b < p.n_seq; b += kPgThreads) {
+    const int slot = kv_slot(p.c, p.slots, p.seq0 + b);
+    const int len = kv_length(p.c, slot);
+    int64_t first;
+    const int rows = kv_rows(p.c, p.cu, p.seq0 + b, p.n_tokens, &first) * p.group;
+    s_slot[b] = slot;
+    s_len[b] = len;
+    s_pre[b] = (rows + kPgRows - 1) / kPgRows * p.c.heads * max((len + kPgKeys - 1) / kPgKeys, 1);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int run = 0;
+    for (int base = 0; base < p.n_seq; base += 32) {
+      const int v = base + lane < p.n_seq ? s_pre[base + lane] : 0;
+      int incl = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+      }
+      if (base + lane < p.n_seq) s_pre[base + lane] = run + incl - v;
+      run += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) s_pre[p.n_seq] = run;
+  }
+  __syncthreads();
+  const PgLists lists{s_pre, s_slot, s_len};
+  const int total = s_pre[p.n_seq];
+  const int per = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  const int lo = min(static_cast<int64_t>(blockIdx.x) * per, static_cast<int64_t>(total));
+  const int hi = min(lo + per, total);
+
+  if (warp == kPgConsumers) {
+    // ------------------------------------------------------------ producer
+    int n = 0;  // tiles issued
+    bool ok = true;
+    for (int x = lo; x < hi && ok;) {
+      const PgItem it = pg_item(p, lists, x, hi);
+      x += it.t1 - it.t0;
+      const int n_keys = it.len;
+      const int first_slice = it.t0 * 4, end_slice = min(it.t1 * 4, (n_keys + 15) >> 4);
+      // Lane i of batch k looks after slice first_slice + 32 k + i.
+      auto page_of = [&](int slice) {
+        return slice < end_slice ? kv_page(p.c, it.slot, (slice << 4) >> p.c.shift) : -1;
+      };
+      int id = page_of(first_slice + lane), id1 = page_of(first_slice + 32 + lane);
+      float ks = 0.0f, vs = 0.0f, ks1 = 0.0f, vs1 = 0.0f;
+      if (id >= 0) {
+        ks = p.c.ks[kv_scale_at(p.c, id, it.head)];
+        vs = p.c.vs[kv_scale_at(p.c, id, it.head)];
+      }
+      for (int base = it.t0; base < it.t1 && ok; base += 8) {
+        const int id2 = page_of((base + 16) * 4 + lane);
+        if (id1 >= 0) {
+          ks1 = p.c.ks[kv_scale_at(p.c, id1, it.head)];
+          vs1 = p.c.vs[kv_scale_at(p.c, id1, it.head)];
+        }
+        const float v1 = vs == 0.0f ? 1.0f : vs;
+        const float4 con = id >= 0 ? make_float4(ks * p.scale_log2, log2f(v1), 1.0f / v1, 1.0f)
+                                   : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+        for (int i = 0; i < 8 && base + i < it.t1; ++i, ++n) {
+          const int s = n % ST;
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((n / ST) & 1u) ^ 1u, p.limit_ns, p.c.err));
+          if (!ok) break;
+          if (lane >> 2 == i) s_const[s * 4 + (lane & 3)] = con;
+          __syncwarp();
+          // One load per page of the tile: by the lane of the page's first slice.
+          const int slice = lane & 3;
+          const int per_page = p.c.shift >= 6 ? 4 : 1 << (p.c.shift - 4);
+          const bool mine = (lane >> 2) == i && id >= 0 && slice % per_page == 0;
+          const unsigned who = __ballot_sync(0xffffffffu, mine);
+          if (lane == 0) {
+            const uint32_t bytes = __popc(who) * per_page * 16 * D * 2;
+            mbar_arrive_expect_tx(&full[s], bytes);
+          }
+          __syncwarp();
+          if (mine) {
+            uint8_t* sk = smem + s * 2 * Cfg::kTile + slice * 16 * D;
+            const int key = (base + i) * kPgKeys + slice * 16;
+            const int off = key & ((1 << p.c.shift) - 1);  // row within the page
+            const int row = ((id * p.c.heads + it.head) << p.c.shift) + off;
+            const int y = D == 128 ? row : row >> 1;
+            tma_load_2d(sk, &tmK, &full[s], 0, y);
+            tma_load_2d(sk + Cfg::kTile, &tmV, &full[s], 0, y);
+          }
+        }
+        id = id1;
+        ks = ks1;
+        vs = vs1;
+        id1 = id2;
+      }
+    }
+    // No copy may still be writing shared memory when the CTA leaves.
+    for (int j = max(n - ST, 0); j < n; ++j) mbar_wait(&full[j % ST], (j / ST) & 1u, p.limit_ns, p.c.err);
   } else {
-    for (int64_t base = 0; base < p.n_seq && b < 0; base += 32) {
-      const int64_t i = base + lane;
-      if (i < p.n_seq) n = kv_rows(p.c, p.cu, i, p.n_tokens, &first);
-      const bool mine = i < p.n_seq && first <= t && t < first + n;
-      const unsigned hit = __ballot_sync(0xffffffffu, mine);
-      if (hit != 0) b = base + __ffs(hit) - 1;
+    // ----------------------------------------------------------- consumers
+    const int g = lane >> 2, t = lane & 3;
+    constexpr int NK = D / 16;  // contraction steps of Q K^T
+    constexpr int NT = D / 8;   // 8-column tiles of the output
+    int n = 0;
+    bool ok = true;
+    if (threadIdx.x == 0) p.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    for (int x = lo; x < hi;) {
+      const PgItem it = pg_item(p, lists, x, hi);
+      x += it.t1 - it.t0;
+      // Query rows g and g + 8: A fragments, the lane's D / 4 elements of a row from t * D / 4.
+      uint32_t aq[NK][4];
+      int lim[NR];
+      int least = it.len;
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const int flat = it.row0 + g + 8 * r;
+        const int tok = flat / p.group;
+        lim[r] = it.len;
+        if (flat < it.n_rows) {
+          const uint4* src = reinterpret_cast<const uint4*>(
+              p.q + (it.first + tok) * p.q_pitch +
+              static_cast<int64_t>(it.head * p.group + flat - tok * p.group) * D + t * (D / 4));
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            const uint4 w = __ldg(src + i);
+            aq[2 * i][r] = w.x;
+            aq[2 * i][r + 2] = w.y;
+            aq[2 * i + 1][r] = w.z;
+            aq[2 * i + 1][r + 2] = w.w;
+          }
+          if (p.causal) lim[r] = it.len - it.n_tok + tok + 1;
+        } else {
+#pragma unroll
+          for (int i = 0; i < NK; ++i) aq[i][r] = aq[i][r + 2] = 0;
+        }
+        least = min(least, lim[r]);
+      }
+      least = __reduce_min_sync(0xffffffffu, least);
+      float o[NT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+      float m[NR], l[NR];
+#pragma unroll
+      for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.0f;
+
+      for (int tile = it.t0; tile < it.t1; ++tile, ++n) {
+        const int s = n % ST;
+        if (ok) ok = mbar_wait(&full[s], (n / ST) & 1u, p.limit_ns, p.c.err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) continue;
+        const uint32_t sk = smem_u32(smem + s * 2 * Cfg::kTile);
+        const uint32_t sv = sk + Cfg::kTile;
+        const int k0 = warp * 16;  // this warp's first key of the tile
+        const float4 con = s_const[s * 4 + warp];
+        float sc[2][4];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
+          const int key = k0 + nt * 8 + g;
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            const uint4 w = lds128(sk + pg_at<D>(key, t * (D / 64) + c));
+            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t b0, b1;
+              codes_to_half4<E4M3>(ws[i], b0, b1);
+              mma16816<R8>(sc[nt], aq[c * 4 + i], b0, b1);
+            }
+          }
+        }
+        // x = S kc + lv; masked keys -inf.
+        const int pos = tile * kPgKeys + k0;
+        float mx[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          mx[r] = -INFINITY;
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float v = fmaf(sc[nt][2 * r + e], con.x, con.y);
+              sc[nt][2 * r + e] = v;
+            }
+          }
+        }
+        if (pos + 16 > least || con.w == 0.0f) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (pos + nt * 8 + 2 * t + e >= lim[r] || con.w == 0.0f) sc[nt][2 * r + e] = -INFINITY;
+            }
+          }
+        }
+        bool grow = false;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          mx[r] = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
+          grow |= mx[r] > m[r] + kPgRescale;
+        }
+        // The reference m follows the running maximum only where that passed it by 2^8
+        // (weights stay below 2^8); the result does not depend on it.
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            float v = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+            v = fmaxf(v, m[r]);
+            const float a = v == -INFINITY ? 1.0f : ex2_approx(m[r] - v);
+            m[r] = v;
+            l[r] *= a;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              o[j][2 * r] *= a;
+              o[j][2 * r + 1] *= a;
+            }
+          }
+        }
+        uint32_t pa[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          const float base = m[r] == -INFINITY ? 0.0f : m[r];
+          float w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = ex2_approx(sc[i >> 1][2 * r + (i & 1)] - base);
+          const float sum = (w[0] + w[1]) + (w[2] + w[3]);
+          l[r] = fmaf(sum, sum != 0.0f ? con.z : 0.0f, l[r]);  // a NaN scale counts only where it is seen
+          const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
+          pa[r] = *reinterpret_cast<const uint32_t*>(&h0);
+          pa[r + 2] = *reinterpret_cast<const uint32_t*>(&h1);
+        }
+        // O += P V: the lane's D / 8 elements, from g * D / 8, of keys 2t, 2t+1, 2t+8, 2t+9.
+        uint32_t v[4][D / 32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = k0 + 2 * t + (i & 1) + 8 * (i >> 1);
+          if constexpr (D == 128) {
+            const uint4 w = lds128(sv + pg_at<D>(key, g));
+            v[i][0] = w.x;
+            v[i][1] = w.y;
+            v[i][2] = w.z;
+            v[i][3] = w.w;
+          } else {
+            const uint2 w = lds64(sv + pg_at<D>(key, g >> 1) + (g & 1) * 8);
+            v[i][0] = w.x;
+            v[i][1] = w.y;
+          }
+          // Bytes that are no sequence's may be e4m3 NaN, which a weight of 0 would not silence.
+          if (E4M3 && (pos + 16 > it.len || con.w == 0.0f)) {
+            const int at = pos + 2 * t + (i & 1) + 8 * (i >> 1);
+            if (at >= it.len || con.w == 0.0f) {
+#pragma unroll
+              for (int j = 0; j < D / 32; ++j) v[i][j] = 0;
+            }
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          uint32_t b0[4], b1[4];
+          codes_to_half4<E4M3>(__byte_perm(v[0][j], v[1][j], 0x5140), b0[0], b0[1]);
+          codes_to_half4<E4M3>(__byte_perm(v[0][j], v[1][j], 0x7362), b0[2], b0[3]);
+          codes_to_half4<E4M3>(__byte_perm(v[2][j], v[3][j], 0x5140), b1[0], b1[1]);
+          codes_to_half4<E4M3>(__byte_perm(v[2][j], v[3][j], 0x7362), b1[2], b1[3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mma16816<R8>(o[j * 4 + e], pa, b0[e], b1[e]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s]);
+      }
+
+      // Join the four warps: (m, l) of each row, then O in warp order.  Element j of
+      // o[.][e] of a lane is column (2t + e) * D / 8 + j.
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        if (t == 0) s_ml[warp * kPgRows + g + 8 * r] = make_float2(m[r], l[r]);
+      }
+      consumer_sync();
+      float a[NR];
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kPgConsumers; ++w) mm = fmaxf(mm, s_ml[w * kPgRows + g + 8 * r].x);
+        a[r] = m[r] == -INFINITY ? (l[r] != l[r] ? l[r] : 0.0f) : ex2_approx(m[r] - mm);
+      }
+      for (int w = 0; w < kPgConsumers; ++w) {
+        if (warp == w) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            float* row = s_o + (g + 8 * r) * D;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+              for (int j = 0; j < NT; j += 4) {
+                float4* dst = reinterpret_cast<float4*>(row + (2 * t + e) * (D / 8) + j);
+                float4 u = w == 0 ? make_float4(0, 0, 0, 0) : *dst;
+                u.x = fmaf(o[j][2 * r + e], a[r], u.x);
+                u.y = fmaf(o[j + 1][2 * r + e], a[r], u.y);
+                u.z = fmaf(o[j + 2][2 * r + e], a[r], u.z);
+                u.w = fmaf(o[j + 3][2 * r + e], a[r], u.w);
+                *dst = u;
+              }
+            }
+          }
+        }
+        consumer_sync();
+      }
+      // 128 threads write the rows, 8 elements each and pass.
+      const bool whole = it.t1 - it.t0 == it.tiles;
+      const int wslot = blockIdx.x * 2 + (it.t0 != 0 ? 0 : 1);
+      constexpr int RT = R8 ? 8 : 16;
+      for (int i = threadIdx.x; i < RT * (D / 8); i += kPgConsumers * 32) {
+        const int row = i / (D / 8), col = (i % (D / 8)) * 8;
+        if (it.row0 + row >= it.n_rows) continue;
+        float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kPgConsumers; ++w) mm = fmaxf(mm, s_ml[w * kPgRows + row].x);
+#pragma unroll
+        for (int w = 0; w < kPgConsumers; ++w) {
+          const float2 e = s_ml[w * kPgRows + row];
+          if (e.x != -INFINITY) ll = fmaf(e.y, ex2_approx(e.x - mm), ll);
+          else if (e.y != e.y) ll = e.y;  // a NaN weight
+        }
+        const float4 u = *reinterpret_cast<const float4*>(s_o + row * D + col);
+        const float4 v = *reinterpret_cast<const float4*>(s_o + row * D + col + 4);
+        if (whole) {
+          if (!ok) continue;
+          const int64_t at = pg_row(p, it.first, it.head, it.row0 + row);
+          const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+          const __half2 h[4] = {__floats2half2_rn(u.x * inv, u.y * inv), __floats2half2_rn(u.z * inv, u.w * inv),
+                                __floats2half2_rn(v.x * inv, v.y * inv), __floats2half2_rn(v.z * inv, v.w * inv)};
+          *reinterpret_cast<uint4*>(p.out + at * D + col) = *reinterpret_cast<const uint4*>(h);
+          if (p.lse != nullptr && col == 0)
+            p.lse[at] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
+        } else {
+          float4* dst = reinterpret_cast<float4*>(p.ws_o + (static_cast<int64_t>(wslot) * kPgRows + row) * D + col);
+          dst[0] = u;
+          dst[1] = v;
+          if (col == 0) p.ws_ml[wslot * kPgRows + row] = make_float2(mm, ll);
+        }
+      }
+      if (threadIdx.x == 0 && it.t0 == 0 && !whole)
+        p.cut[blockIdx.x] = make_int4(it.b, it.row0, it.head, (it.begin + it.tiles - 1) / per);
+      consumer_sync();  // s_o and s_ml are free again
     }
-    if (b < 0) return;
-    n = kv_rows(p.c, p.cu, b, p.n_tokens, &first);
   }
-  const int slot = kv_slot(p.c, p.slots, b);
-  const int len = kv_length(p.c, slot);
-  const int last = p.causal ? len - n + static_cast<int>(t - first) : len - 1;
-  constexpr int E = D / 32;
-  const int kvh = h / (p.n_heads / p.c.heads);
-  float q[E], o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = __half2float(p.q[t * p.q_pitch + static_cast<int64_t>(h) * D + lane * E + e]);
-    o[e] = 0.0f;
+}
+
+/// Joins the parts of the item that CTA blockIdx.x of attn_paged_kernel began and did
+/// not finish (its part 1, and part 0 of each CTA up to the one that finished it);
+/// blockIdx.y is the row, thread i has column i.
+template <int D>
+__global__ void __launch_bounds__(D) attn_paged_join_kernel(const ApParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int4 cut = p.cut[blockIdx.x];
+  if (cut.x < 0) return;
+  const int row = blockIdx.y, col = threadIdx.x;
+  int64_t first;
+  const int n_rows = kv_rows(p.c, p.cu, p.seq0 + cut.x, p.n_tokens, &first) * p.group;
+  if (cut.y + row >= n_rows) return;
+  const int parts = cut.w - static_cast<int>(blockIdx.x) + 1;
+  const int part0 = 2 * static_cast<int>(blockIdx.x);
+  auto slot = [&](int i) { return static_cast<int64_t>(part0 + (i == 0 ? 1 : 2 * i)) * kPgRows + row; };
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) m = fmaxf(m, p.ws_ml[slot(i)].x);
+  float l = 0.0f, o = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const float2 ml = p.ws_ml[slot(i)];
+    // A part without a visible key has m = -inf, l = 0 and o = 0 (or NaN in all: kept).
+    const float a = ml.x == -INFINITY ? 1.0f : ex2_approx(ml.x - m);
+    l = fmaf(ml.y, a, l);
+    o = fmaf(p.ws_o[slot(i) * D + col], a, o);
   }
-  float m = -INFINITY, l = 0.0f;
-  auto code = [](uint8_t v) {
-    uint32_t lo, hi;
-    codes_to_half4<E4M3>(v, lo, hi);
-    return __half2float(__low2half(*reinterpret_cast<__half2*>(&lo)));
-  };
-  const int page = 1 << p.c.shift;
-  for (int e0 = 0; e0 * page <= last; ++e0) {
-    const int id = kv_page(p.c, slot, e0);
-    if (id < 0) continue;
-    const float ks = p.c.ks[kv_scale_at(p.c, id, kvh)] * p.scale_log2;
-    float vs = p.c.vs[kv_scale_at(p.c, id, kvh)];
-    if (vs == 0.0f) vs = 1.0f;
-    const float lv = log2f(vs), iv = 1.0f / vs;
-    const int64_t tile = kv_tile<D>(p.c, id, kvh);
-    for (int j = 0; j < page && e0 * page + j <= last; ++j) {
-      const uint8_t* kr = p.c.k + tile + j * D + lane * E;
-      const uint8_t* vr = p.c.v + tile + j * D + lane * E;
-      float s = 0.0f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) s = fmaf(q[e], code(kr[e]), s);
-#pragma unroll
-      for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-      const float x = fmaf(s, ks, lv);
-      const float m_new = fmaxf(m, x);
-      const float base = m_new == -INFINITY ? 0.0f : m_new;
-      const float a = exp2f(m - base), w = exp2f(x - base);
-      l = fmaf(w, iv, l * a);
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(w, code(vr[e]), o[e] * a);
-      m = m_new;
-    }
-  }
+  const int64_t at = pg_row(p, first, cut.z, cut.y + row);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    p.out[(t * p.n_heads + h) * D + lane * E + e] = __float2half_rn(o[e] * inv);
-  if (p.lse != nullptr && lane == 0)
-    p.lse[t * p.n_heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  p.out[at * D + col] = __float2half_rn(o * inv);
+  if (p.lse != nullptr && col == 0)
+    p.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
-template <int D, bool E4M3>
-int launch_simple(const ApParams& p, cudaStream_t st) {
-  const int64_t blocks = (p.n_tokens * p.n_heads + 3) / 4;
-  B200_CUDA(launch_pdl(attn_paged_simple_kernel<D, E4M3>, dim3(static_cast<unsigned>(blocks)), dim3(128),
-                       0, st, p));
-  return ENGINE_OK;
+template <int D, bool E4M3, bool R8>
+int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most_tiles, cudaStream_t st) {
+  using Cfg = PgCfg<D>;
+  auto kern = attn_paged_kernel<D, E4M3, R8>;
+  const size_t smem = Cfg::smem(p.n_seq);
+  static std::atomic<uint64_t> configured{0};
+  int dev = 0;
+  B200_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if ((configured.load() & bit) == 0) {
+    B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   static_cast<int>(Cfg::smem(kPgMaxSeq))));
+    configured.fetch_or(bit);
+  }
+  CUtensorMap tk, tv;
+  const uint64_t rows = static_cast<uint64_t>(kv->n_pages * kv->n_kv_heads * kv->page_size) * D / 128;
+  const uint32_t box = static_cast<uint32_t>(kv->page_size < kPgKeys ? kv->page_size : kPgKeys) * D / 128;
+  if (!make_tmap_2d(&tk, p.c.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, 128, 128, box, 128) ||
+      !make_tmap_2d(&tv, p.c.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, 128, 128, box, 128))
+    return ENGINE_ERR_CUDA;
+  // Three CTAs an SM while their shared memory fits (up to about 100 sequences).
+  const int64_t per_sm = std::min<int64_t>(3, (max_smem_optin() + 1024) / static_cast<int64_t>(smem + 1024));
+  const int64_t ctas = std::min<int64_t>(sm_count() * std::max<int64_t>(per_sm, 1), most_tiles);
+  const size_t o_bytes = 2 * ctas * kPgRows * D * sizeof(float), ml_bytes = 2 * ctas * kPgRows * sizeof(float2);
+  char* ws = static_cast<char*>(scratch_alloc(o_bytes + ml_bytes + ctas * sizeof(int4), st));
+  if (ws == nullptr) return set_error(ENGINE_ERR_CUDA, "attention_paged: workspace allocation failed");
+  p.ws_o = reinterpret_cast<float*>(ws);
+  p.ws_ml = reinterpret_cast<float2*>(ws + o_bytes);
+  p.cut = reinterpret_cast<int4*>(ws + o_bytes + ml_bytes);
+  int rc = ENGINE_OK;
+  cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPgThreads), smem, st, tk, tv, p);
+  if (e == cudaSuccess)
+    e = launch_pdl(attn_paged_join_kernel<D>, dim3(static_cast<unsigned>(ctas), R8 ? 8 : 16), dim3(D), 0, st, p);
+  if (e != cudaSuccess) rc = set_cuda_error(e, "attn_paged_kernel");
+  scratch_free(ws, st);
+  return rc;
 }
 
-int run_paged(const ApParams& p, const engine_kv_pages_t* kv, cudaStream_t st, const char* what) {
+/// The sequences, in launches of at most kPgMaxSeq.
+int run_paged(ApParams p, const engine_kv_pages_t* kv, int64_t n_seq, cudaStream_t st, const char* what) {
   const bool e4m3 = kv->type == ENGINE_KV_E4M3;
-  int rc;
-  if (kv->head_dim == 64) rc = e4m3 ? launch_simple<64, true>(p, st) : launch_simple<64, false>(p, st);
-  else rc = e4m3 ? launch_simple<128, true>(p, st) : launch_simple<128, false>(p, st);
-  if (rc != ENGINE_OK) return rc;
+  const int64_t tiles = std::max<int64_t>((kv->max_pages * kv->page_size + kPgKeys - 1) / kPgKeys, 1);
+  const bool r8 = p.cu == nullptr && p.group <= 8;
+  for (int64_t at = 0; at < n_seq; at += kPgMaxSeq) {
+    const int64_t n = std::min<int64_t>(kPgMaxSeq, n_seq - at);
+    // At most this many tiles (the kernel counts them in 32 bits).
+    const int64_t groups = p.cu == nullptr ? n * ((p.group + kPgRows - 1) / kPgRows)
+                                           : p.n_tokens * p.group / kPgRows + n;
+    if (groups > 0x7fffffff / kv->n_kv_heads / tiles)
+      return set_error(ENGINE_ERR_UNSUPPORTED, std::string(what) + ": too many query rows x positions");
+    p.seq0 = static_cast<int>(at);
+    p.n_seq = static_cast<int>(n);
+    const int64_t most = groups * kv->n_kv_heads * tiles;
+    int rc;
+    if (kv->head_dim == 64) {
+      rc = e4m3 ? (r8 ? launch_paged<64, true, true>(p, kv, most, st) : launch_paged<64, true, false>(p, kv, most, st))
+                : (r8 ? launch_paged<64, false, true>(p, kv, most, st) : launch_paged<64, false, false>(p, kv, most, st));
+    } else {
+      rc = e4m3 ? (r8 ? launch_paged<128, true, true>(p, kv, most, st) : launch_paged<128, true, false>(p, kv, most, st))
+                : (r8 ? launch_paged<128, false, true>(p, kv, most, st) : launch_paged<128, false, false>(p, kv, most, st));
+    }
+    if (rc != ENGINE_OK) return rc;
+  }
   return check_launch(what);
 }
 
@@ -150,6 +692,26 @@ int check_paged(const engine_kv_pages_t* kv, int64_t layer, const void* q, int64
   return ENGINE_OK;
 }
 
+ApParams paged_params(const engine_kv_pages_t* kv, int64_t layer, const engine_half_t* q,
+                      int64_t q_pitch, const int32_t* slots, const int32_t* cu, engine_half_t* out,
+                      float* lse, int64_t n_tokens, int64_t n_heads, float scale, bool causal) {
+  ApParams p = {};
+  p.c = kv_view(kv, layer);
+  p.q = reinterpret_cast<const __half*>(q);
+  p.q_pitch = q_pitch;
+  p.slots = slots;
+  p.cu = cu;
+  p.out = reinterpret_cast<__half*>(out);
+  p.lse = lse;
+  p.n_tokens = n_tokens;
+  p.n_heads = static_cast<int>(n_heads);
+  p.group = static_cast<int>(n_heads / kv->n_kv_heads);
+  p.causal = causal ? 1 : 0;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.limit_ns = wait_limit_ns();
+  return p;
+}
+
 }  // namespace
 }  // namespace b200
 
@@ -167,19 +729,9 @@ int engine_cuda_attention_paged_decode(const engine_kv_pages_t* kv, int64_t laye
   if (const int rc = check_paged(kv, layer, q, q_pitch, slots, out, n_seq, n_seq, n_heads, scale, what))
     return rc;
   if (n_seq == 0) return ENGINE_OK;
-  const ApParams p{kv_view(kv, layer),
-                   reinterpret_cast<const __half*>(q),
-                   q_pitch,
-                   slots,
-                   nullptr,
-                   reinterpret_cast<__half*>(out),
-                   out_lse,
-                   n_seq,
-                   n_seq,
-                   static_cast<int>(n_heads),
-                   0,
-                   scale * 1.4426950408889634f};
-  return run_paged(p, kv, static_cast<cudaStream_t>(stream), what);
+  const ApParams p = paged_params(kv, layer, q, q_pitch, slots, nullptr, out, out_lse, n_seq, n_heads,
+                                  scale, false);
+  return run_paged(p, kv, n_seq, static_cast<cudaStream_t>(stream), what);
   B200_ENTRY_END
 }
 
@@ -196,19 +748,9 @@ int engine_cuda_attention_paged_prefill(const engine_kv_pages_t* kv, int64_t lay
     return rc;
   if (n_seq == 0 || n_tokens == 0) return ENGINE_OK;
   B200_REQUIRE(cu_q != nullptr, "attention_paged_prefill: cu_q is null");
-  const ApParams p{kv_view(kv, layer),
-                   reinterpret_cast<const __half*>(q),
-                   q_pitch,
-                   slots,
-                   cu_q,
-                   reinterpret_cast<__half*>(out),
-                   out_lse,
-                   n_seq,
-                   n_tokens,
-                   static_cast<int>(n_heads),
-                   is_causal != 0 ? 1 : 0,
-                   scale * 1.4426950408889634f};
-  return run_paged(p, kv, static_cast<cudaStream_t>(stream), what);
+  const ApParams p = paged_params(kv, layer, q, q_pitch, slots, cu_q, out, out_lse, n_tokens, n_heads,
+                                  scale, is_causal != 0);
+  return run_paged(p, kv, n_seq, static_cast<cudaStream_t>(stream), what);
   B200_ENTRY_END
 }
 
