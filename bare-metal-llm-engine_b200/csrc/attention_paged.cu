@@ -21,13 +21,14 @@
 // and scales, 32 slices of 16 keys at a time and one batch ahead, and fetches each
 // tile's K and V codes by TMA into a ring of kStages x 64 keys (rows of 128 bytes,
 // 128-byte swizzle); each consumer warp owns 16 keys of every tile.
-//   Products: mma.sync m16n8k16 with the query rows as A.  tcgen05 would want its
-// operands as FP16 in shared memory, and writing the widened codes there and back
-// costs more than the products (16 rows x 16 keys x 2 d FLOP against 16 x 2 d
-// bytes); here a lane turns the bytes that it has just loaded into B fragments in
-// registers.  The order of the contraction is free, so a lane's B elements are
-// consecutive bytes: D / 4 of one key's row for Q K^T, D / 8 of four keys' rows for
-// P V.  S comes out in the layout that P V wants as its A operand.
+//   Products: mma.sync m16n8k16 with the keys (later the elements of the values) as
+// A's 16 rows and the query rows as B's 8 columns: S^T = K q^T, O^T += V^T P^T, so
+// eight rows cost one instruction where q as A would fill half of it.  tcgen05 would
+// want its operands as FP16 in shared memory, and writing the widened codes there and
+// back costs more than the products.  Here a lane turns the bytes that it has just
+// loaded into A fragments in registers.  The order of the contraction is free, so they
+// are consecutive bytes: D / 4 of two keys' rows for S^T, D / 8 of four keys' rows for
+// O^T; P passes from one layout to the other by two 8 x 8 transpositions.
 
 #include <algorithm>
 #include <atomic>
@@ -40,7 +41,7 @@ namespace b200 {
 namespace {
 
 constexpr int kPgKeys = 64;      // keys per tile
-constexpr int kPgRows = 16;      // query rows per item
+constexpr int kPgRows = 16;      // query rows per item, at most
 constexpr int kPgConsumers = 4;  // warps; each takes 16 keys of a tile
 constexpr int kPgThreads = (kPgConsumers + 1) * 32;
 constexpr int kPgMaxSeq = 1024;  // sequences per launch (their prefix sums sit in shared memory)
@@ -65,15 +66,20 @@ struct ApParams {
   unsigned long long limit_ns;
 };
 
-template <int D>
+/// NQ: groups of 8 query rows of an item.  One: 3 CTAs an SM with 128 registers a
+/// thread; two need about 170: 2 CTAs.
+template <int D, int NQ>
 struct PgCfg {
+  static constexpr int kRows = 8 * NQ;
+  static constexpr int kCtas = NQ == 1 ? 3 : 2;
   static constexpr int kTile = kPgKeys * D;  // bytes of K (or V) of a tile
-  static constexpr int kStages = D == 128 ? 4 : 6;
+  static constexpr int kStages = (NQ == 1 ? 4 : 6) * (D == 128 ? 2 : 3) / 2;
+  static constexpr int kOW = D + 4;          // pitch of a row of O in shared memory
   static constexpr int kOffO = kStages * 2 * kTile;
-  static constexpr int kOffConst = kOffO + kPgRows * D * 4;
+  static constexpr int kOffConst = kOffO + kRows * kOW * 4;
   static constexpr int kOffBar = kOffConst + kStages * 4 * 16;
   static constexpr int kOffMl = kOffBar + 2 * kStages * 8;
-  static constexpr int kOffSeq = kOffMl + kPgConsumers * kPgRows * 8;
+  static constexpr int kOffSeq = kOffMl + kPgConsumers * kRows * 8;
   static size_t smem(int n_seq) { return kOffSeq + 12 * (static_cast<size_t>(n_seq) + 1) + 1024; }
 };
 
@@ -83,26 +89,40 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
-/// d += a b, m16n8k16.  With R8, rows 8..15 of a are zero and of d unused.  The whole
-/// warp has to come here together: callers put __syncwarp() behind code that the lanes'
-/// rows may branch in (a row's own branch around its sum lost parts of O).
-template <bool R8>
+/// d += a b, m16n8k16.  The whole warp has to come here together: callers put
+/// __syncwarp() behind code that the lanes' rows may branch in.
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (R8) {
-    float x, y;
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, "
-        "{%0, %1, %9, %9};"
-        : "+f"(d[0]), "+f"(d[1]), "=f"(x), "=f"(y)
-        : "r"(a[0]), "r"(0), "r"(a[2]), "r"(b0), "r"(b1), "f"(0.0f));
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+/// The 8 x 8 transpose of a matrix of 16-bit elements, two of row lane / 4 in each lane.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+/// Four codes of a key as the two fragment registers of a contraction step.  e4m3:
+/// bytes (0, 1) and (2, 3), exactly.  int8: bytes (0, 2) and (1, 3) as the FP16
+/// subnormals (q + 128) 2^-24 -- the byte itself, its sign bit flipped, in a 16-bit
+/// lane: 3 instructions for 4 codes, 5 where the 128 is taken off here.  It is taken
+/// off the sums instead, which start at -128 2^-24 sum(q) (below full scale of the
+/// codes, so it costs the FP32 sums no more than their largest values do).  P V cannot
+/// do so: there the sum over thousands of keys can be far below the offset's.
+template <bool E4M3>
+__device__ __forceinline__ void k_fragment(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (E4M3) {
+    codes_to_half4<true>(w, lo, hi);
   } else {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    lo = (w & 0x00ff00ffu) ^ 0x00800080u;
+    hi = __byte_perm(w, 0, 0x4341) ^ 0x00800080u;
   }
 }
+constexpr float kKeyUnit = 5.9604644775390625e-8f;  // 2^-24
 
 /// Shared-memory offset, within a tile, of the 16 bytes `c` of key `key`'s row.
 template <int D>
@@ -113,17 +133,6 @@ __device__ __forceinline__ uint32_t pg_at(int key, int c) {
     const int line = key >> 1;
     return line * 128 + (((((key & 1) << 2) | c) ^ (line & 7)) << 4);
   }
-}
-
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-  return v;
 }
 
 /// Barrier of the consumer warps.  bar.sync wants whole warps: lanes that parted
@@ -184,13 +193,12 @@ __device__ __forceinline__ int64_t pg_row(const ApParams& p, int64_t first, int 
   return (first + tok) * p.n_heads + head * p.group + (flat - tok * p.group);
 }
 
-template <int D, bool E4M3, bool R8>
-__global__ void __launch_bounds__(kPgThreads, 3)
+template <int D, bool E4M3, int NQ>
+__global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
     attn_paged_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                       const ApParams p) {
-  using Cfg = PgCfg<D>;
+  using Cfg = PgCfg<D, NQ>;
   constexpr int ST = Cfg::kStages;
-  constexpr int NR = R8 ? 1 : 2;  // query rows per lane: g and g + 8
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -250,6 +258,7 @@ __global__ void __launch_bounds__(kPgThreads, 3)
 
   if (warp == kPgConsumers) {
     // ------------------------------------------------------------ producer
+    const float kc_unit = p.scale_log2 * (E4M3 ? 1.0f : 1.0f / kKeyUnit);
     int n = 0;  // tiles issued
     bool ok = true;
     for (int x = lo; x < hi && ok;) {
@@ -274,7 +283,7 @@ __global__ void __launch_bounds__(kPgThreads, 3)
           vs1 = p.c.vs[kv_scale_at(p.c, id1, it.head)];
         }
         const float v1 = vs == 0.0f ? 1.0f : vs;
-        const float4 con = id >= 0 ? make_float4(ks * p.scale_log2, log2f(v1), 1.0f / v1, 1.0f)
+        const float4 con = id >= 0 ? make_float4(ks * kc_unit, log2f(v1), 1.0f / v1, 1.0f)
                                    : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
         for (int i = 0; i < 8 && base + i < it.t1; ++i, ++n) {
           const int s = n % ST;
@@ -313,211 +322,245 @@ __global__ void __launch_bounds__(kPgThreads, 3)
   } else {
     // ----------------------------------------------------------- consumers
     const int g = lane >> 2, t = lane & 3;
-    constexpr int NK = D / 16;  // contraction steps of Q K^T
-    constexpr int NT = D / 8;   // 8-column tiles of the output
+    constexpr int NK = D / 16;  // contraction steps of S^T, and 16-row tiles of O^T
     int n = 0;
     bool ok = true;
     if (threadIdx.x == 0) p.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
     for (int x = lo; x < hi;) {
       const PgItem it = pg_item(p, lists, x, hi);
       x += it.t1 - it.t0;
-      // Query rows g and g + 8: A fragments, the lane's D / 4 elements of a row from t * D / 4.
-      uint32_t aq[NK][4];
-      int lim[NR];
+      // q^T as B fragments: the lane's D / 4 elements of query row g (and g + 8), from
+      // t * D / 4.  In the sums' columns a lane has rows 2t and 2t + 1 (and + 8).
+      uint32_t bq[NQ][NK][2];
+      float init[NQ][2];
+      int lim[NQ][2];
       int least = it.len;
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        const int flat = it.row0 + g + 8 * r;
-        const int tok = flat / p.group;
-        lim[r] = it.len;
-        if (flat < it.n_rows) {
-          const uint4* src = reinterpret_cast<const uint4*>(
-              p.q + (it.first + tok) * p.q_pitch +
-              static_cast<int64_t>(it.head * p.group + flat - tok * p.group) * D + t * (D / 4));
+      for (int nq = 0; nq < NQ; ++nq) {
+        const int flat = it.row0 + 8 * nq + g;
+        const bool row = flat < it.n_rows;
+        const uint4* src = reinterpret_cast<const uint4*>(
+            p.q + (it.first + (row ? flat / p.group : 0)) * p.q_pitch +
+            static_cast<int64_t>(it.head * p.group + (row ? flat % p.group : 0)) * D + t * (D / 4));
+        float sum = 0.0f;
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            const uint4 w = __ldg(src + i);
-            aq[2 * i][r] = w.x;
-            aq[2 * i][r + 2] = w.y;
-            aq[2 * i + 1][r] = w.z;
-            aq[2 * i + 1][r + 2] = w.w;
+        for (int i = 0; i < NK / 2; ++i) {
+          const uint4 w = row ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+          const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t u0 = q[2 * e], u1 = q[2 * e + 1];
+            if constexpr (E4M3) {
+              bq[nq][2 * i + e][0] = u0;
+              bq[nq][2 * i + e][1] = u1;
+            } else {  // elements (0, 2) and (1, 3), as k_fragment pairs the codes
+              bq[nq][2 * i + e][0] = __byte_perm(u0, u1, 0x5410);
+              bq[nq][2 * i + e][1] = __byte_perm(u0, u1, 0x7632);
+              const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&u0));
+              const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&u1));
+              sum += (f0.x + f0.y) + (f1.x + f1.y);
+            }
           }
-          if (p.causal) lim[r] = it.len - it.n_tok + tok + 1;
-        } else {
-#pragma unroll
-          for (int i = 0; i < NK; ++i) aq[i][r] = aq[i][r + 2] = 0;
         }
-        least = min(least, lim[r]);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          init[nq][e] = -128.0f * kKeyUnit * __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4);
+          const int f = it.row0 + 8 * nq + 2 * t + e;
+          lim[nq][e] = it.len;
+          if (p.causal && f < it.n_rows) lim[nq][e] = it.len - it.n_tok + f / p.group + 1;
+          least = min(least, lim[nq][e]);
+        }
       }
       least = __reduce_min_sync(0xffffffffu, least);
-      float o[NT][4];
+      float o[NQ][NK][4];
+      float m[NQ][2], l[NQ][2];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-      float m[NR], l[NR];
+      for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
-      for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.0f;
+        for (int j = 0; j < NK; ++j) o[nq][j][0] = o[nq][j][1] = o[nq][j][2] = o[nq][j][3] = 0.0f;
+        m[nq][0] = m[nq][1] = -INFINITY;
+        l[nq][0] = l[nq][1] = 0.0f;
+      }
 
       for (int tile = it.t0; tile < it.t1; ++tile, ++n) {
         const int s = n % ST;
         if (ok) ok = mbar_wait(&full[s], (n / ST) & 1u, p.limit_ns, p.c.err);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) continue;
-        const uint32_t sk = smem_u32(smem + s * 2 * Cfg::kTile);
-        const uint32_t sv = sk + Cfg::kTile;
+        const uint8_t* sk = smem + s * 2 * Cfg::kTile;
+        const uint8_t* sv = sk + Cfg::kTile;
         const int k0 = warp * 16;  // this warp's first key of the tile
         const float4 con = s_const[s * 4 + warp];
-        float sc[2][4];
+        // S^T: keys g and g + 8 in rows, element [nq][0..3] = (g, 2t) (g, 2t+1) (g+8, 2t) (g+8, 2t+1).
+        uint32_t kw[2][NK];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
-          const int key = k0 + nt * 8 + g;
+        for (int r = 0; r < 2; ++r) {
 #pragma unroll
-          for (int c = 0; c < D / 64; ++c) {
-            const uint4 w = lds128(sk + pg_at<D>(key, t * (D / 64) + c));
-            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t b0, b1;
-              codes_to_half4<E4M3>(ws[i], b0, b1);
-              mma16816<R8>(sc[nt], aq[c * 4 + i], b0, b1);
-            }
-          }
+          for (int c = 0; c < D / 64; ++c)
+            *reinterpret_cast<uint4*>(&kw[r][4 * c]) =
+                *reinterpret_cast<const uint4*>(sk + pg_at<D>(k0 + 8 * r + g, t * (D / 64) + c));
         }
-        // x = S kc + lv; masked keys -inf.
+        float sc[NQ][4];
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[nq][e] = E4M3 ? 0.0f : init[nq][e & 1];
+        }
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          uint32_t a[4];
+          k_fragment<E4M3>(kw[0][i], a[0], a[2]);
+          k_fragment<E4M3>(kw[1][i], a[1], a[3]);
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq) mma16816(sc[nq], a, bq[nq][i][0], bq[nq][i][1]);
+        }
+        // The lane's D / 8 elements, from g * D / 8, of keys 2t, 2t+1, 2t+8, 2t+9: on their way
+        // while the weights are formed.
         const int pos = tile * kPgKeys + k0;
-        float mx[NR];
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          mx[r] = -INFINITY;
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float v = fmaf(sc[nt][2 * r + e], con.x, con.y);
-              sc[nt][2 * r + e] = v;
-            }
-          }
-        }
-        if (pos + 16 > least || con.w == 0.0f) {
-#pragma unroll
-          for (int r = 0; r < NR; ++r) {
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (pos + nt * 8 + 2 * t + e >= lim[r] || con.w == 0.0f) sc[nt][2 * r + e] = -INFINITY;
-            }
-          }
-        }
-        bool grow = false;
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          mx[r] = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
-          grow |= mx[r] > m[r] + kPgRescale;
-        }
-        // The reference m follows the running maximum only where that passed it by 2^8
-        // (weights stay below 2^8); the result does not depend on it.
-        if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            float v = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-            v = fmaxf(v, m[r]);
-            const float a = v == -INFINITY ? 1.0f : ex2_approx(m[r] - v);
-            m[r] = v;
-            l[r] *= a;
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              o[j][2 * r] *= a;
-              o[j][2 * r + 1] *= a;
-            }
-          }
-        }
-        uint32_t pa[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          const float base = m[r] == -INFINITY ? 0.0f : m[r];
-          float w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = ex2_approx(sc[i >> 1][2 * r + (i & 1)] - base);
-          const float sum = (w[0] + w[1]) + (w[2] + w[3]);
-          l[r] = fmaf(sum, sum != 0.0f ? con.z : 0.0f, l[r]);  // a NaN scale counts only where it is seen
-          const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
-          pa[r] = *reinterpret_cast<const uint32_t*>(&h0);
-          pa[r + 2] = *reinterpret_cast<const uint32_t*>(&h1);
-        }
-        // O += P V: the lane's D / 8 elements, from g * D / 8, of keys 2t, 2t+1, 2t+8, 2t+9.
         uint32_t v[4][D / 32];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = k0 + 2 * t + (i & 1) + 8 * (i >> 1);
           if constexpr (D == 128) {
-            const uint4 w = lds128(sv + pg_at<D>(key, g));
-            v[i][0] = w.x;
-            v[i][1] = w.y;
-            v[i][2] = w.z;
-            v[i][3] = w.w;
+            *reinterpret_cast<uint4*>(v[i]) = *reinterpret_cast<const uint4*>(sv + pg_at<D>(key, g));
           } else {
-            const uint2 w = lds64(sv + pg_at<D>(key, g >> 1) + (g & 1) * 8);
-            v[i][0] = w.x;
-            v[i][1] = w.y;
+            *reinterpret_cast<uint2*>(v[i]) =
+                *reinterpret_cast<const uint2*>(sv + pg_at<D>(key, g >> 1) + (g & 1) * 8);
           }
-          // Bytes that are no sequence's may be e4m3 NaN, which a weight of 0 would not silence.
-          if (E4M3 && (pos + 16 > it.len || con.w == 0.0f)) {
-            const int at = pos + 2 * t + (i & 1) + 8 * (i >> 1);
-            if (at >= it.len || con.w == 0.0f) {
+        }
+        // x = S kc + lv; masked keys -inf.
 #pragma unroll
-              for (int j = 0; j < D / 32; ++j) v[i][j] = 0;
+        for (int nq = 0; nq < NQ; ++nq) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[nq][e] = fmaf(sc[nq][e], con.x, con.y);
+        }
+        if (pos + 16 > least || con.w == 0.0f) {
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (pos + g + 8 * (e >> 1) >= lim[nq][e & 1] || con.w == 0.0f) sc[nq][e] = -INFINITY;
+          }
+          if (E4M3) {  // bytes that are no sequence's may be NaN, which a weight of 0 would not silence
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool none = pos + 2 * t + (i & 1) + 8 * (i >> 1) >= it.len || con.w == 0.0f;
+#pragma unroll
+              for (int j = 0; j < D / 32; ++j) v[i][j] = none ? 0u : v[i][j];
             }
           }
         }
+        bool grow = false;
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) grow |= fmaxf(sc[nq][e], sc[nq][e + 2]) > m[nq][e] + kPgRescale;
+        }
+        // The reference m follows the running maximum only where that passed it by 2^8
+        // (weights stay below 2^8); the result does not depend on it.
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float u = fmaxf(sc[nq][e], sc[nq][e + 2]);
+#pragma unroll
+              for (int w = 4; w < 32; w <<= 1) u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, w));
+              u = fmaxf(u, m[nq][e]);
+              const float a = u == -INFINITY ? 1.0f : ex2_approx(m[nq][e] - u);
+              m[nq][e] = u;
+              l[nq][e] *= a;
+#pragma unroll
+              for (int j = 0; j < NK; ++j) {
+                o[nq][j][e] *= a;
+                o[nq][j][e + 2] *= a;
+              }
+            }
+          }
+        }
+        uint32_t bp[NQ][2];
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float base = m[nq][e & 1] == -INFINITY ? 0.0f : m[nq][e & 1];
+            w[e] = ex2_approx(sc[nq][e] - base);
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float sum = w[e] + w[e + 2];
+            // a NaN scale counts only where it is seen
+            l[nq][e] = fmaf(sum, sum != 0.0f ? con.z : 0.0f, l[nq][e]);
+          }
+          const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
+          bp[nq][0] = *reinterpret_cast<const uint32_t*>(&h0);
+          bp[nq][1] = *reinterpret_cast<const uint32_t*>(&h1);
+        }
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-          uint32_t b0[4], b1[4];
-          codes_to_half4<E4M3>(__byte_perm(v[0][j], v[1][j], 0x5140), b0[0], b0[1]);
-          codes_to_half4<E4M3>(__byte_perm(v[0][j], v[1][j], 0x7362), b0[2], b0[3]);
-          codes_to_half4<E4M3>(__byte_perm(v[2][j], v[3][j], 0x5140), b1[0], b1[1]);
-          codes_to_half4<E4M3>(__byte_perm(v[2][j], v[3][j], 0x7362), b1[2], b1[3]);
+        for (int nq = 0; nq < NQ; ++nq) {
+          bp[nq][0] = transpose8x8(bp[nq][0]);
+          bp[nq][1] = transpose8x8(bp[nq][1]);
+        }
+        // O^T: 16-row tile i has elements g * D / 8 + 2i (row g) and + 2i + 1 (row g + 8).
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mma16816<R8>(o[j * 4 + e], pa, b0[e], b1[e]);
+        for (int j = 0; j < D / 32; ++j) {
+          uint32_t lo[4], hi[4];  // of the four bytes: keys 2t, 2t+1 and keys 2t+8, 2t+9
+          codes_to_half4<E4M3>(__byte_perm(v[0][j], v[1][j], 0x5140), lo[0], lo[1]);
+          codes_to_half4<E4M3>(__byte_perm(v[0][j], v[1][j], 0x7362), lo[2], lo[3]);
+          codes_to_half4<E4M3>(__byte_perm(v[2][j], v[3][j], 0x5140), hi[0], hi[1]);
+          codes_to_half4<E4M3>(__byte_perm(v[2][j], v[3][j], 0x7362), hi[2], hi[3]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t a[4] = {lo[2 * e], lo[2 * e + 1], hi[2 * e], hi[2 * e + 1]};
+#pragma unroll
+            for (int nq = 0; nq < NQ; ++nq) mma16816(o[nq][2 * j + e], a, bp[nq][0], bp[nq][1]);
+          }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[s]);
       }
 
-      // Join the four warps: (m, l) of each row, then O in warp order.  Element j of
-      // o[.][e] of a lane is column (2t + e) * D / 8 + j.
+      // Join the four warps: (m, l) of each row, then O in warp order.
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        if (t == 0) s_ml[warp * kPgRows + g + 8 * r] = make_float2(m[r], l[r]);
+      for (int nq = 0; nq < NQ; ++nq) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) l[nq][e] += __shfl_xor_sync(0xffffffffu, l[nq][e], w);
+          if (g == 0) s_ml[warp * Cfg::kRows + 8 * nq + 2 * t + e] = make_float2(m[nq][e], l[nq][e]);
+        }
       }
       consumer_sync();
-      float a[NR];
+      float a[NQ][2];
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        float mm = -INFINITY;
+      for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
-        for (int w = 0; w < kPgConsumers; ++w) mm = fmaxf(mm, s_ml[w * kPgRows + g + 8 * r].x);
-        a[r] = m[r] == -INFINITY ? (l[r] != l[r] ? l[r] : 0.0f) : ex2_approx(m[r] - mm);
+        for (int e = 0; e < 2; ++e) {
+          float mm = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < kPgConsumers; ++w) mm = fmaxf(mm, s_ml[w * Cfg::kRows + 8 * nq + 2 * t + e].x);
+          a[nq][e] = m[nq][e] == -INFINITY ? (l[nq][e] != l[nq][e] ? l[nq][e] : 0.0f) : ex2_approx(m[nq][e] - mm);
+        }
       }
       for (int w = 0; w < kPgConsumers; ++w) {
         if (warp == w) {
 #pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            float* row = s_o + (g + 8 * r) * D;
+          for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+              float* row = s_o + (8 * nq + 2 * t + e) * Cfg::kOW + g * (D / 8);
 #pragma unroll
-              for (int j = 0; j < NT; j += 4) {
-                float4* dst = reinterpret_cast<float4*>(row + (2 * t + e) * (D / 8) + j);
+              for (int j = 0; j < NK; j += 2) {
+                float4* dst = reinterpret_cast<float4*>(row + 2 * j);
                 float4 u = w == 0 ? make_float4(0, 0, 0, 0) : *dst;
-                u.x = fmaf(o[j][2 * r + e], a[r], u.x);
-                u.y = fmaf(o[j + 1][2 * r + e], a[r], u.y);
-                u.z = fmaf(o[j + 2][2 * r + e], a[r], u.z);
-                u.w = fmaf(o[j + 3][2 * r + e], a[r], u.w);
+                u.x = fmaf(o[nq][j][e], a[nq][e], u.x);
+                u.y = fmaf(o[nq][j][e + 2], a[nq][e], u.y);
+                u.z = fmaf(o[nq][j + 1][e], a[nq][e], u.z);
+                u.w = fmaf(o[nq][j + 1][e + 2], a[nq][e], u.w);
                 *dst = u;
               }
             }
@@ -525,37 +568,32 @@ __global__ void __launch_bounds__(kPgThreads, 3)
         }
         consumer_sync();
       }
-      // 128 threads write the rows, 8 elements each and pass.
+      // The rows go out, 4 elements a thread and pass.
       const bool whole = it.t1 - it.t0 == it.tiles;
       const int wslot = blockIdx.x * 2 + (it.t0 != 0 ? 0 : 1);
-      constexpr int RT = R8 ? 8 : 16;
-      for (int i = threadIdx.x; i < RT * (D / 8); i += kPgConsumers * 32) {
-        const int row = i / (D / 8), col = (i % (D / 8)) * 8;
+      for (int i = threadIdx.x; i < Cfg::kRows * (D / 4); i += kPgConsumers * 32) {
+        const int row = i / (D / 4), col = (i % (D / 4)) * 4;
         if (it.row0 + row >= it.n_rows) continue;
         float mm = -INFINITY, ll = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kPgConsumers; ++w) mm = fmaxf(mm, s_ml[w * kPgRows + row].x);
+        for (int w = 0; w < kPgConsumers; ++w) mm = fmaxf(mm, s_ml[w * Cfg::kRows + row].x);
 #pragma unroll
         for (int w = 0; w < kPgConsumers; ++w) {
-          const float2 e = s_ml[w * kPgRows + row];
+          const float2 e = s_ml[w * Cfg::kRows + row];
           if (e.x != -INFINITY) ll = fmaf(e.y, ex2_approx(e.x - mm), ll);
           else if (e.y != e.y) ll = e.y;  // a NaN weight
         }
-        const float4 u = *reinterpret_cast<const float4*>(s_o + row * D + col);
-        const float4 v = *reinterpret_cast<const float4*>(s_o + row * D + col + 4);
+        const float4 u = *reinterpret_cast<const float4*>(s_o + row * Cfg::kOW + col);
         if (whole) {
           if (!ok) continue;
           const int64_t at = pg_row(p, it.first, it.head, it.row0 + row);
           const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-          const __half2 h[4] = {__floats2half2_rn(u.x * inv, u.y * inv), __floats2half2_rn(u.z * inv, u.w * inv),
-                                __floats2half2_rn(v.x * inv, v.y * inv), __floats2half2_rn(v.z * inv, v.w * inv)};
-          *reinterpret_cast<uint4*>(p.out + at * D + col) = *reinterpret_cast<const uint4*>(h);
+          const __half2 h[2] = {__floats2half2_rn(u.x * inv, u.y * inv), __floats2half2_rn(u.z * inv, u.w * inv)};
+          *reinterpret_cast<uint2*>(p.out + at * D + col) = *reinterpret_cast<const uint2*>(h);
           if (p.lse != nullptr && col == 0)
             p.lse[at] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
         } else {
-          float4* dst = reinterpret_cast<float4*>(p.ws_o + (static_cast<int64_t>(wslot) * kPgRows + row) * D + col);
-          dst[0] = u;
-          dst[1] = v;
+          *reinterpret_cast<float4*>(p.ws_o + (static_cast<int64_t>(wslot) * kPgRows + row) * D + col) = u;
           if (col == 0) p.ws_ml[wslot * kPgRows + row] = make_float2(mm, ll);
         }
       }
@@ -601,10 +639,10 @@ __global__ void __launch_bounds__(D) attn_paged_join_kernel(const ApParams p) {
     p.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
-template <int D, bool E4M3, bool R8>
+template <int D, bool E4M3, int NQ>
 int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most_tiles, cudaStream_t st) {
-  using Cfg = PgCfg<D>;
-  auto kern = attn_paged_kernel<D, E4M3, R8>;
+  using Cfg = PgCfg<D, NQ>;
+  auto kern = attn_paged_kernel<D, E4M3, NQ>;
   const size_t smem = Cfg::smem(p.n_seq);
   static std::atomic<uint64_t> configured{0};
   int dev = 0;
@@ -621,8 +659,8 @@ int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most_tiles, cu
   if (!make_tmap_2d(&tk, p.c.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, 128, 128, box, 128) ||
       !make_tmap_2d(&tv, p.c.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, 128, 128, box, 128))
     return ENGINE_ERR_CUDA;
-  // Three CTAs an SM while their shared memory fits (up to about 100 sequences).
-  const int64_t per_sm = std::min<int64_t>(3, (max_smem_optin() + 1024) / static_cast<int64_t>(smem + 1024));
+  // kCtas an SM while their shared memory fits (three: up to about 300 sequences).
+  const int64_t per_sm = std::min<int64_t>(Cfg::kCtas, (max_smem_optin() + 1024) / static_cast<int64_t>(smem + 1024));
   const int64_t ctas = std::min<int64_t>(sm_count() * std::max<int64_t>(per_sm, 1), most_tiles);
   const size_t o_bytes = 2 * ctas * kPgRows * D * sizeof(float), ml_bytes = 2 * ctas * kPgRows * sizeof(float2);
   char* ws = static_cast<char*>(scratch_alloc(o_bytes + ml_bytes + ctas * sizeof(int4), st));
@@ -633,7 +671,7 @@ int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most_tiles, cu
   int rc = ENGINE_OK;
   cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPgThreads), smem, st, tk, tv, p);
   if (e == cudaSuccess)
-    e = launch_pdl(attn_paged_join_kernel<D>, dim3(static_cast<unsigned>(ctas), R8 ? 8 : 16), dim3(D), 0, st, p);
+    e = launch_pdl(attn_paged_join_kernel<D>, dim3(static_cast<unsigned>(ctas), Cfg::kRows), dim3(D), 0, st, p);
   if (e != cudaSuccess) rc = set_cuda_error(e, "attn_paged_kernel");
   scratch_free(ws, st);
   return rc;
@@ -656,11 +694,11 @@ int run_paged(ApParams p, const engine_kv_pages_t* kv, int64_t n_seq, cudaStream
     const int64_t most = groups * kv->n_kv_heads * tiles;
     int rc;
     if (kv->head_dim == 64) {
-      rc = e4m3 ? (r8 ? launch_paged<64, true, true>(p, kv, most, st) : launch_paged<64, true, false>(p, kv, most, st))
-                : (r8 ? launch_paged<64, false, true>(p, kv, most, st) : launch_paged<64, false, false>(p, kv, most, st));
+      rc = e4m3 ? (r8 ? launch_paged<64, true, 1>(p, kv, most, st) : launch_paged<64, true, 2>(p, kv, most, st))
+                : (r8 ? launch_paged<64, false, 1>(p, kv, most, st) : launch_paged<64, false, 2>(p, kv, most, st));
     } else {
-      rc = e4m3 ? (r8 ? launch_paged<128, true, true>(p, kv, most, st) : launch_paged<128, true, false>(p, kv, most, st))
-                : (r8 ? launch_paged<128, false, true>(p, kv, most, st) : launch_paged<128, false, false>(p, kv, most, st));
+      rc = e4m3 ? (r8 ? launch_paged<128, true, 1>(p, kv, most, st) : launch_paged<128, true, 2>(p, kv, most, st))
+                : (r8 ? launch_paged<128, false, 1>(p, kv, most, st) : launch_paged<128, false, 2>(p, kv, most, st));
     }
     if (rc != ENGINE_OK) return rc;
   }
