@@ -34,8 +34,7 @@
 #include <atomic>
 #include <cmath>
 
-#include "kernels.cuh"
-#include "kv_pages.cuh"
+#include "attention_paged.cuh"
 
 namespace b200 {
 namespace {
@@ -46,25 +45,8 @@ constexpr int kPgConsumers = 4;  // warps; each takes 16 keys of a tile
 constexpr int kPgThreads = (kPgConsumers + 1) * 32;
 constexpr int kPgMaxSeq = 1024;  // sequences per launch (their prefix sums sit in shared memory)
 constexpr float kPgRescale = 8.0f;
-
-struct ApParams {
-  KvView c;
-  const __half* q;
-  int64_t q_pitch;
-  const int32_t* slots;
-  const int32_t* cu;  // null: one row per sequence
-  __half* out;
-  float* lse;
-  int seq0, n_seq;    // sequences [seq0, seq0 + n_seq) of the call
-  int64_t n_tokens;
-  int n_heads, group;
-  int causal;
-  float scale_log2;
-  float* ws_o;        // [2 * CTAs][rows][D]
-  float2* ws_ml;      // [2 * CTAs][rows]
-  int4* cut;          // [CTAs]: the item that a CTA began and did not finish
-  unsigned long long limit_ns;
-};
+constexpr int64_t kManyRows = 32;  // from here on attention_paged_tc
+static_assert(kPgMaxSeq <= kTcMaxSeq, "both kernels take a launch's sequences");
 
 /// NQ: groups of 8 query rows of an item.  One: 3 CTAs an SM with 128 registers a
 /// thread; two need about 170: 2 CTAs.
@@ -82,12 +64,6 @@ struct PgCfg {
   static constexpr int kOffSeq = kOffMl + kPgConsumers * kRows * 8;
   static size_t smem(int n_seq) { return kOffSeq + 12 * (static_cast<size_t>(n_seq) + 1) + 1024; }
 };
-
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 /// d += a b, m16n8k16.  The whole warp has to come here together: callers put
 /// __syncwarp() behind code that the lanes' rows may branch in.
@@ -682,6 +658,8 @@ int run_paged(ApParams p, const engine_kv_pages_t* kv, int64_t n_seq, cudaStream
   const bool e4m3 = kv->type == ENGINE_KV_E4M3;
   const int64_t tiles = std::max<int64_t>((kv->max_pages * kv->page_size + kPgKeys - 1) / kPgKeys, 1);
   const bool r8 = p.cu == nullptr && p.group <= 8;
+  // Rows per sequence and KV head, on the average (the host knows no more).
+  const bool many = p.cu != nullptr && p.group <= 128 && p.n_tokens * p.group >= kManyRows * n_seq;
   for (int64_t at = 0; at < n_seq; at += kPgMaxSeq) {
     const int64_t n = std::min<int64_t>(kPgMaxSeq, n_seq - at);
     // At most this many tiles (the kernel counts them in 32 bits).
@@ -691,6 +669,10 @@ int run_paged(ApParams p, const engine_kv_pages_t* kv, int64_t n_seq, cudaStream
       return set_error(ENGINE_ERR_UNSUPPORTED, std::string(what) + ": too many query rows x positions");
     p.seq0 = static_cast<int>(at);
     p.n_seq = static_cast<int>(n);
+    if (many) {
+      if (const int rc = attention_paged_tc(p, kv, st)) return rc;
+      continue;
+    }
     const int64_t most = groups * kv->n_kv_heads * tiles;
     int rc;
     if (kv->head_dim == 64) {
