@@ -662,17 +662,17 @@ int run_paged(ApParams p, const engine_kv_pages_t* kv, int64_t n_seq, cudaStream
   const bool many = p.cu != nullptr && p.group <= 128 && p.n_tokens * p.group >= kManyRows * n_seq;
   for (int64_t at = 0; at < n_seq; at += kPgMaxSeq) {
     const int64_t n = std::min<int64_t>(kPgMaxSeq, n_seq - at);
-    // At most this many tiles (the kernel counts them in 32 bits).
-    const int64_t groups = p.cu == nullptr ? n * ((p.group + kPgRows - 1) / kPgRows)
-                                           : p.n_tokens * p.group / kPgRows + n;
-    if (groups > 0x7fffffff / kv->n_kv_heads / tiles)
-      return set_error(ENGINE_ERR_UNSUPPORTED, std::string(what) + ": too many query rows x positions");
     p.seq0 = static_cast<int>(at);
     p.n_seq = static_cast<int>(n);
     if (many) {
       if (const int rc = attention_paged_tc(p, kv, st)) return rc;
       continue;
     }
+    // At most this many tiles (the kernel counts them in 32 bits).
+    const int64_t groups = p.cu == nullptr ? n * ((p.group + kPgRows - 1) / kPgRows)
+                                           : p.n_tokens * p.group / kPgRows + n;
+    if (groups > 0x7fffffff / kv->n_kv_heads / tiles)
+      return set_error(ENGINE_ERR_UNSUPPORTED, std::string(what) + ": too many query rows x positions");
     const int64_t most = groups * kv->n_kv_heads * tiles;
     int rc;
     if (kv->head_dim == 64) {

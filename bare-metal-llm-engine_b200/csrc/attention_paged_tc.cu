@@ -16,7 +16,8 @@
 // (m, l, O) in a workspace, and a second kernel joins the parts in order.
 //   Warps: 0-3 widen codes (TMA'd bytes in, swizzled FP16 operand tiles out, two
 // stages each of K and V); 4-7 and 8-11 are the softmax of side A and B, one thread
-// per row; 12 looks up pages and scales and issues the TMA; 13 issues the MMAs.
+// per row; 12 looks up pages and scales and issues the TMA; 13 issues the MMAs; 14 and
+// 15 only share their warpgroup's register split.
 //   TMEM: S of A and B (128 columns each, overwritten by P as FP16 pairs) and O of A
 // and B.  The MMA warp alternates the sides -- P V of the last tile, then S of the
 // next -- so that one side's softmax runs under the other side's products.
@@ -32,7 +33,7 @@
 namespace b200 {
 namespace {
 
-constexpr int kTcThreads = 448;
+constexpr int kTcThreads = 512;
 constexpr int kTcKeys = 128;
 constexpr int kTcRows = 256;  // two sides
 constexpr float kTcRescale = 8.0f;
@@ -138,6 +139,41 @@ __device__ TcItem tc_find(const TcParams& p, const int32_t* pre, int x, int hi) 
   return it;
 }
 
+// Registers a thread: 128 at launch (65536 / 512); the softmax warps take from the rest
+// (128 * 96 + 256 * 168 + 128 * 80 = 65536).
+constexpr int kRegsWiden = 96, kRegsSoftmax = 168, kRegsOther = 80;
+static_assert(128 * kRegsWiden + 256 * kRegsSoftmax + 128 * kRegsOther <= 65536, "register split");
+template <int N>
+__device__ __forceinline__ void set_max_regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void set_max_regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+/// Two FP32 lanes to an instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 struct TcBars {
   uint64_t q_full, q_empty;
   uint64_t raw_full[2], raw_empty[2];  // K, V
@@ -199,24 +235,35 @@ __device__ __forceinline__ float tc_row_weights(uint32_t tS, const float4* con, 
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float4 c = con[c4 * 2 + h];
-      const float off = c.y - base;
-      float s0 = 0.0f, s1 = 0.0f;
+      const uint64_t kc = pack2(c.x, c.x), off = pack2(c.y - base, c.y - base);
+      float2 w[8];
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        float p0 = ex2_approx(fmaf(__uint_as_float(v[h * 16 + e]), c.x, off));
-        float p1 = ex2_approx(fmaf(__uint_as_float(v[h * 16 + e + 1]), c.x, off));
+      for (int e = 0; e < 8; ++e)
+        w[e] = unpack2(fma2(pack2(__uint_as_float(v[h * 16 + 2 * e]), __uint_as_float(v[h * 16 + 2 * e + 1])), kc, off));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        w[e].x = ex2_approx(w[e].x);
+        w[e].y = ex2_approx(w[e].y);
         if (MASK) {
-          const int k = k0 + (c4 * 2 + h) * 16 + e;
-          if (k >= lim || c.w == 0.0f) p0 = 0.0f;
-          if (k + 1 >= lim || c.w == 0.0f) p1 = 0.0f;
+          const int k = k0 + (c4 * 2 + h) * 16 + 2 * e;
+          if (k >= lim || c.w == 0.0f) w[e].x = 0.0f;
+          if (k + 1 >= lim || c.w == 0.0f) w[e].y = 0.0f;
         }
-        s0 += p0;
-        s1 += p1;
-        const __half2 u = __floats2half2_rn(p0, p1);
-        pk[h * 8 + (e >> 1)] = *reinterpret_cast<const uint32_t*>(&u);
       }
-      const float s = s0 + s1;
-      l = fmaf(s, s != 0.0f ? c.z : 0.0f, l);  // a NaN scale counts only where it is seen
+      uint64_t s0 = pack2(w[0].x, w[0].y), s1 = pack2(w[1].x, w[1].y);
+#pragma unroll
+      for (int e = 2; e < 8; e += 2) {
+        s0 = add2(s0, pack2(w[e].x, w[e].y));
+        s1 = add2(s1, pack2(w[e + 1].x, w[e + 1].y));
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const __half2 u = __floats2half2_rn(w[e].x, w[e].y);
+        pk[h * 8 + e] = *reinterpret_cast<const uint32_t*>(&u);
+      }
+      const float2 t = unpack2(add2(s0, s1));
+      const float sum = t.x + t.y;
+      l = fmaf(sum, sum != 0.0f ? c.z : 0.0f, l);  // a NaN scale counts only where it is seen
     }
     tmem_st_32x32b_x16(tS + c4 * 16, pk);
   }
@@ -231,7 +278,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  float4* s_const = reinterpret_cast<float4*>(smem + Cfg::kOffConst);  // [4 tiles][8 slices]
+  // [4 tiles][8 slices of 16 keys]: ks scale log2 e, log2 vs, 1 / vs, and whether the
+  // slice has a page (0: no; 2: the tile's eight slices all have)
+  float4* s_const = reinterpret_cast<float4*>(smem + Cfg::kOffConst);
   TcBars* bar = reinterpret_cast<TcBars*>(smem + Cfg::kOffBar);
   int32_t* s_pre = reinterpret_cast<int32_t*>(smem + Cfg::kOffRaw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -306,6 +355,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (warp < 4) {
     // ------------------------------------------------------------- widening
+    set_max_regs_dec<kRegsWiden>();
     int n = 0;
     bool ok = true;
     for (int x = lo; x < hi && ok;) {
@@ -339,9 +389,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                   raw + line * 128 + (((((key[i] & 1) << 2) | ch[i]) ^ (line & 7)) << 4));
             }
           }
-          if (E4M3 && kv) {
+          const float4* con = s_const + (n & 3) * 8;
+          if (E4M3 && kv && ((t + 1) * kTcKeys > it.len || con[0].w != 2.0f)) {
             // Bytes that are no sequence's may be NaN, which a weight of 0 would not silence.
-            const float4* con = s_const + (n & 3) * 8;
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
               if (t * kTcKeys + key[i] >= it.len || con[key[i] >> 4].w == 0.0f) w[i] = make_uint4(0, 0, 0, 0);
@@ -372,6 +422,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   } else if (warp < 12) {
     // -------------------------------------------------------------- softmax
+    set_max_regs_inc<kRegsSoftmax>();
     const int side = (warp - 4) >> 2;
     const int r = (warp & 3) * 32 + lane;  // row of the side's tile, TMEM lane
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -390,10 +441,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_after();
         const float4* con = s_const + (n & 3) * 8;
         const int k0 = t * kTcKeys;
-        float good = con[0].w;
-#pragma unroll
-        for (int i = 1; i < 8; ++i) good = fminf(good, con[i].w);
-        const bool clean = __all_sync(0xffffffffu, k0 + kTcKeys <= lim && good != 0.0f);
+        const bool clean = __all_sync(0xffffffffu, k0 + kTcKeys <= lim && con[0].w == 2.0f);
         const float mt = clean ? tc_row_max<false>(tS, con, k0, lim) : tc_row_max<true>(tS, con, k0, lim);
         // Lazy rescaling: the row keeps its reference until the maximum passes it by 2^8.
         const bool first = m == -INFINITY;
@@ -461,6 +509,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (x < hi) tc_next(p, it, x, hi);
     }
   } else {
+    set_max_regs_dec<kRegsOther>();
     if (warp == 12) {
       // ----------------------------------------------------- lookups and TMA
       int n = 0, items = 0;
@@ -498,16 +547,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (vs == 0.0f) vs = 1.0f;
             con = make_float4(ks * p.a.scale_log2, log2f(vs), 1.0f / vs, 1.0f);
           }
+          const unsigned valid = __ballot_sync(0xffffffffu, id >= 0);
           for (int i = 0; i < 4 && base + i < it.t1 && ok; ++i, ++n) {
             const int slice = lane & 7;
             const bool mine = (lane >> 3) == i && id >= 0 && slice % per_box == 0;
             const unsigned who = __ballot_sync(0xffffffffu, mine);
+            float4 con_i = con;
+            if (((valid >> (8 * i)) & 0xffu) == 0xffu) con_i.w = 2.0f;
             const int key = (base + i) * kTcKeys + slice * 16;
             const int row = mine ? ((id * c.heads + it.head) << c.shift) + (key & ((1 << c.shift) - 1)) : 0;
             for (int kv = 0; kv < 2; ++kv) {
               ok = __all_sync(0xffffffffu, mbar_wait(&bar->raw_empty[kv], (n & 1) ^ 1u, limit, c.err));
               if (!ok) break;
-              if (kv == 0 && (lane >> 3) == i) s_const[(n & 3) * 8 + slice] = con;
+              if (kv == 0 && (lane >> 3) == i) s_const[(n & 3) * 8 + slice] = con_i;
               __syncwarp();
               if (lane == 0) mbar_arrive_expect_tx(&bar->raw_full[kv], __popc(who) * per_box * 16 * D);
               __syncwarp();
