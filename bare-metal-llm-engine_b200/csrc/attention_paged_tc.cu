@@ -15,28 +15,29 @@
 // per SM, whatever the lengths are (they are on the device).  Items that are cut leave
 // (m, l, O) in a workspace, and a second kernel joins the parts in order.
 //   Warps: 0-3 widen codes (TMA'd bytes in, swizzled FP16 operand tiles out, two
-// stages each of K and V); 4-7 and 8-11 are the softmax of side A and B, one thread
-// per row; 12 looks up pages and scales and issues the TMA; 13 issues the MMAs; 14 and
-// 15 only share their warpgroup's register split.
+// stages each of K and V); 4-11 and 12-19 are the softmax of side A and B, four threads
+// to a row; 20 looks up pages and scales and issues the TMA; 21 and 22 issue the MMAs of
+// side A and B; 23 only shares its warpgroup's register split.
 //   TMEM: S of A and B (128 columns each, overwritten by P as FP16 pairs) and O of A
-// and B.  The MMA warp alternates the sides -- P V of the last tile, then S of the
-// next -- so that one side's softmax runs under the other side's products.
+// and B.  Within a side, S -> softmax -> P V is a chain; the two sides' chains interleave
+// on the tensor cores and the exponential units.
 //
 // Every wait is bounded (ENGINE_WAIT_TIMEOUT_MS): on expiry the thread sets the device
 // error word, its role ends, the others' waits run out too, and all meet at the
 // teardown, where copies and MMAs in flight are waited for.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "attention_paged.cuh"
 
 namespace b200 {
 namespace {
 
-constexpr int kTcThreads = 512;
+constexpr int kTcThreads = 768;
 constexpr int kTcKeys = 128;
 constexpr int kTcRows = 256;  // two sides
-constexpr float kTcRescale = 8.0f;
+constexpr float kTcRescale = 14.0f;  // weights stay below 2^14 (FP16 ends at 2^16)
 
 template <int D>
 struct TcCfg {
@@ -61,12 +62,17 @@ struct TcParams {
   int tq;  // tokens per side
 };
 
+/// What an item costs beside its key tiles (its Q, the first tile's chain, O's way out;
+/// about 7000 cycles against 4000 a tile), in tiles: the even shares count it, as steps in
+/// front of the item's tiles in which nothing is done.
+constexpr int kTcItemCost = 2;
+
 struct TcItem {
-  int b, slot, len, n_tok;
+  int b, slot, len, n_tok, nb;  // nb: the sequence's items per head
   int64_t first;
   int head, qb;
   int t0, t1, tiles;
-  int begin;  // the item's first tile, counted over all items
+  int begin;  // the item's first step, counted over all items
 };
 
 __device__ __forceinline__ int tc_tiles(const TcParams& p, int len, int n_tok, int qb) {
@@ -80,12 +86,20 @@ __device__ __forceinline__ void tc_sequence(const TcParams& p, int b, TcItem& it
   it.slot = kv_slot(p.a.c, p.a.slots, p.a.seq0 + b);
   it.len = kv_length(p.a.c, it.slot);
   it.n_tok = kv_rows(p.a.c, p.a.cu, p.a.seq0 + b, p.a.n_tokens, &it.first);
+  it.nb = (it.n_tok + 2 * p.tq - 1) / (2 * p.tq);
 }
 
-/// Moves on to the item after `it`, whose first tile is at `x` (< the total).
+/// The tiles that the steps from x on, before hi, have of the item.
+__device__ __forceinline__ void tc_range(TcItem& it, int x, int hi) {
+  it.t0 = max(x - it.begin - kTcItemCost, 0);
+  it.t1 = max(min(hi - it.begin - kTcItemCost, it.tiles), it.t0);
+}
+/// The step behind the item's part.
+__device__ __forceinline__ int tc_end(const TcItem& it) { return it.begin + kTcItemCost + it.t1; }
+
+/// Moves on to the item after `it`, whose first step is x (< the total).
 __device__ __forceinline__ void tc_next(const TcParams& p, TcItem& it, int x, int hi) {
-  const int nb = (it.n_tok + 2 * p.tq - 1) / (2 * p.tq);
-  if (++it.qb >= nb) {
+  if (++it.qb >= it.nb) {
     it.qb = 0;
     if (++it.head >= p.a.c.heads) {
       it.head = 0;
@@ -96,11 +110,10 @@ __device__ __forceinline__ void tc_next(const TcParams& p, TcItem& it, int x, in
   }
   it.begin = x;
   it.tiles = tc_tiles(p, it.len, it.n_tok, it.qb);
-  it.t0 = 0;
-  it.t1 = min(it.tiles, hi - x);
+  tc_range(it, x, hi);
 }
 
-/// The item at tile x, found by the whole warp.  pre: tiles before each sequence.
+/// The item at step x, found by the whole warp.  pre: steps before each sequence.
 __device__ TcItem tc_find(const TcParams& p, const int32_t* pre, int x, int hi) {
   TcItem it;
   int lo = 0, up = p.a.n_seq - 1;
@@ -113,11 +126,10 @@ __device__ TcItem tc_find(const TcParams& p, const int32_t* pre, int x, int hi) 
   const int per_head = (pre[lo + 1] - pre[lo]) / p.a.c.heads;
   const int y = x - pre[lo];
   it.head = y / per_head;
-  int z = y - it.head * per_head;  // tile among the head's
-  const int nb = (it.n_tok + 2 * p.tq - 1) / (2 * p.tq);
-  for (int base = 0; base < nb; base += 32) {
+  int z = y - it.head * per_head;  // step among the head's
+  for (int base = 0; base < it.nb; base += 32) {
     const int qb = base + static_cast<int>(lane_id());
-    const int v = qb < nb ? tc_tiles(p, it.len, it.n_tok, qb) : 0;
+    const int v = qb < it.nb ? kTcItemCost + tc_tiles(p, it.len, it.n_tok, qb) : 0;
     int incl = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -128,21 +140,20 @@ __device__ TcItem tc_find(const TcParams& p, const int32_t* pre, int x, int hi) 
     if (over != 0) {
       const int src = __ffs(over) - 1;
       it.qb = base + src;
-      it.tiles = __shfl_sync(0xffffffffu, v, src);
-      it.t0 = z - __shfl_sync(0xffffffffu, incl - v, src);
+      it.tiles = __shfl_sync(0xffffffffu, v, src) - kTcItemCost;
+      it.begin = x - (z - __shfl_sync(0xffffffffu, incl - v, src));
       break;
     }
     z -= __shfl_sync(0xffffffffu, incl, 31);
   }
-  it.t1 = min(it.tiles, it.t0 + hi - x);
-  it.begin = x - it.t0;
+  tc_range(it, x, hi);
   return it;
 }
 
-// Registers a thread: 128 at launch (65536 / 512); the softmax warps take from the rest
-// (128 * 96 + 256 * 168 + 128 * 80 = 65536).
-constexpr int kRegsWiden = 96, kRegsSoftmax = 168, kRegsOther = 80;
-static_assert(128 * kRegsWiden + 256 * kRegsSoftmax + 128 * kRegsOther <= 65536, "register split");
+// Registers a thread: 80 at launch (65536 / 768, in eights); the softmax warps take from
+// the rest (128 * 72 + 512 * 88 + 128 * 56 = 768 * 80).
+constexpr int kRegsWiden = 72, kRegsSoftmax = 88, kRegsOther = 56;
+static_assert(128 * kRegsWiden + 512 * kRegsSoftmax + 128 * kRegsOther <= kTcThreads * 80, "register split");
 template <int N>
 __device__ __forceinline__ void set_max_regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -178,99 +189,106 @@ struct TcBars {
   uint64_t q_full, q_empty;
   uint64_t raw_full[2], raw_empty[2];  // K, V
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];  // stages
-  uint64_t s_full[2], p_full[2], o_done[2], o_free[2];    // sides
-  uint64_t drain;
+  uint64_t s_full[2], p_full[2][2];                       // sides, halves of 64 keys
+  uint64_t o_done[2], o_free[2], drain[2];                // sides
   uint32_t tmem;
 };
 
-/// A row's maximum of x + log2 vs over a tile, S read from TMEM 32 columns at a time
-/// (the next 32 on their way meanwhile).  MASK: keys from lim on and slices without a
-/// page are left out.
-template <bool MASK>
-__device__ __forceinline__ float tc_row_max(uint32_t tS, const float4* con, int k0, int lim) {
-  float mt = -INFINITY;
-  uint32_t sv[2][32];
-  tmem_ld_32x32b_x32(tS, sv[0]);
+/// A softmax warp has 16 rows of a side; a thread two of them (lane / 4 and + 8) and, of
+/// every 8 columns, 2 (lane % 4) and the next: 32 values of a half tile of 64 keys, in
+/// v[4 (column / 8) + 2 r + {0, 1}].  KG keys share their constants.
+///
+/// tc_half_load reads S.  In a tile that masks something (`clean` false) it makes x + log2 vs
+/// of it, -inf from key lim[r] on; con_of then gives the constants that leave that alone.
+template <int KG>
+__device__ __forceinline__ void tc_half_load(uint32_t taddr, const float4* con, int key, const int (&lim)[2],
+                                             bool clean, uint32_t (&v)[32]) {
+  tmem_ld_16x256b_x8(taddr, v);
+  tmem_wait_ld();
+  if (!clean) {
 #pragma unroll
-  for (int c4 = 0; c4 < 4; ++c4) {
-    tmem_wait_ld();
-    if (c4 < 3) tmem_ld_32x32b_x32(tS + (c4 + 1) * 32, sv[(c4 + 1) & 1]);
-    const uint32_t(&v)[32] = sv[c4 & 1];
+    for (int j = 0; j < 8; ++j) {
+      const float4 c = con[j / 2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float4 c = con[c4 * 2 + h];
-      if (!MASK) {
-        float m0 = -INFINITY, m1 = -INFINITY;
+      for (int r = 0; r < 2; ++r) {
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          m0 = fmaxf(m0, __uint_as_float(v[h * 16 + e]));
-          m1 = fmaxf(m1, __uint_as_float(v[h * 16 + e + 1]));
-        }
-        mt = fmaxf(mt, fmaf(fmaxf(m0, m1), c.x, c.y));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float x = fmaf(__uint_as_float(v[h * 16 + e]), c.x, c.y);
-          if (k0 + (c4 * 2 + h) * 16 + e < lim && c.w != 0.0f) mt = fmaxf(mt, x);
+        for (int e = 0; e < 2; ++e) {
+          const float x = fmaf(__uint_as_float(v[4 * j + 2 * r + e]), c.x, c.y);
+          v[4 * j + 2 * r + e] = __float_as_uint(key + 8 * j + e < lim[r] ? x : -INFINITY);
         }
       }
     }
+    __syncwarp();
   }
-  return mt;
+}
+__device__ __forceinline__ float4 con_of(const float4& c, bool clean) {
+  return clean ? c : make_float4(1.0f, 0.0f, c.z, c.w);
 }
 
-/// The row's weights against the reference `base`, written over S as FP16 pairs (P's
-/// columns trail those still to be read); returns the sum of w / vs.
-template <bool MASK>
-__device__ __forceinline__ float tc_row_weights(uint32_t tS, const float4* con, int k0, int lim, float base) {
-  float l = 0.0f;
-  uint32_t sv[2][32];
-  tmem_ld_32x32b_x32(tS, sv[0]);
+/// The rows' maxima of x + log2 vs.
+template <int KG>
+__device__ __forceinline__ void tc_half_max(const uint32_t (&v)[32], const float4* con, bool clean, float (&mt)[2]) {
 #pragma unroll
-  for (int c4 = 0; c4 < 4; ++c4) {
-    tmem_wait_ld();
-    if (c4 < 3) tmem_ld_32x32b_x32(tS + (c4 + 1) * 32, sv[(c4 + 1) & 1]);
-    const uint32_t(&v)[32] = sv[c4 & 1];
-    uint32_t pk[16];
+  for (int gi = 0; gi < 64 / KG; ++gi) {
+    const float4 c = con_of(con[gi * (KG / 16)], clean);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float4 c = con[c4 * 2 + h];
-      const uint64_t kc = pack2(c.x, c.x), off = pack2(c.y - base, c.y - base);
-      float2 w[8];
+    for (int r = 0; r < 2; ++r) {
+      float mx = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        w[e] = unpack2(fma2(pack2(__uint_as_float(v[h * 16 + 2 * e]), __uint_as_float(v[h * 16 + 2 * e + 1])), kc, off));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        w[e].x = ex2_approx(w[e].x);
-        w[e].y = ex2_approx(w[e].y);
-        if (MASK) {
-          const int k = k0 + (c4 * 2 + h) * 16 + 2 * e;
-          if (k >= lim || c.w == 0.0f) w[e].x = 0.0f;
-          if (k + 1 >= lim || c.w == 0.0f) w[e].y = 0.0f;
-        }
-      }
-      uint64_t s0 = pack2(w[0].x, w[0].y), s1 = pack2(w[1].x, w[1].y);
-#pragma unroll
-      for (int e = 2; e < 8; e += 2) {
-        s0 = add2(s0, pack2(w[e].x, w[e].y));
-        s1 = add2(s1, pack2(w[e + 1].x, w[e + 1].y));
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const __half2 u = __floats2half2_rn(w[e].x, w[e].y);
-        pk[h * 8 + e] = *reinterpret_cast<const uint32_t*>(&u);
-      }
-      const float2 t = unpack2(add2(s0, s1));
-      const float sum = t.x + t.y;
-      l = fmaf(sum, sum != 0.0f ? c.z : 0.0f, l);  // a NaN scale counts only where it is seen
+      for (int j = gi * (KG / 8); j < (gi + 1) * (KG / 8); ++j)
+        mx = fmaxf(mx, fmaxf(__uint_as_float(v[4 * j + 2 * r]), __uint_as_float(v[4 * j + 2 * r + 1])));
+      mt[r] = fmaxf(mt[r], fmaf(mx, c.x, c.y));
     }
-    tmem_st_32x32b_x16(tS + c4 * 16, pk);
   }
-  return l;
 }
 
-template <int D, bool E4M3>
+/// The weights against the references m, as FP16 pairs in the order of
+/// tmem_st_16x128b_x8; adds the thread's w / vs to l.
+template <int KG>
+__device__ __forceinline__ void tc_half_weights(const uint32_t (&v)[32], const float4* con, bool clean,
+                                                const float (&m)[2], float (&l)[2], uint32_t (&pk)[16]) {
+#pragma unroll
+  for (int gi = 0; gi < 64 / KG; ++gi) {
+    const float4 c = con_of(con[gi * (KG / 16)], clean);
+    const uint64_t kc = pack2(c.x, c.x);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float d = c.y - (m[r] == -INFINITY ? 0.0f : m[r]);
+      const uint64_t off = pack2(d, d);
+      uint64_t sum = 0;
+#pragma unroll
+      for (int j = gi * (KG / 8); j < (gi + 1) * (KG / 8); ++j) {
+        float2 w = unpack2(fma2(pack2(__uint_as_float(v[4 * j + 2 * r]), __uint_as_float(v[4 * j + 2 * r + 1])), kc, off));
+        w.x = ex2_approx(w.x);
+        w.y = ex2_approx(w.y);
+        sum = add2(sum, pack2(w.x, w.y));
+        const __half2 u = __floats2half2_rn(w.x, w.y);
+        pk[2 * j + r] = *reinterpret_cast<const uint32_t*>(&u);
+      }
+      const float2 s2 = unpack2(sum);
+      const float s = s2.x + s2.y;
+      l[r] = fmaf(s, s != 0.0f ? c.z : 0.0f, l[r]);  // a NaN scale counts only where it is seen
+    }
+  }
+}
+
+/// 4 x 4 transpose over the four lanes of a row: lane t's r[j] goes to lane j's r[t].
+__device__ __forceinline__ void transpose4(uint32_t (&r)[4], int t) {
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {  // with lane t ^ 1
+    const uint32_t u = __shfl_xor_sync(0xffffffffu, (t & 1) ? r[i] : r[i + 1], 1);
+    if (t & 1) r[i] = u;
+    else r[i + 1] = u;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {  // with lane t ^ 2
+    const uint32_t u = __shfl_xor_sync(0xffffffffu, (t & 2) ? r[i] : r[i + 2], 2);
+    if (t & 2) r[i] = u;
+    else r[i + 2] = u;
+  }
+}
+
+template <int D, bool E4M3, int KG>
 __global__ void __launch_bounds__(kTcThreads, 1)
     attn_paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                          const __grid_constant__ CUtensorMap tmV, const TcParams p) {
@@ -289,38 +307,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(&bar->q_full, 1);
-    mbar_init(&bar->q_empty, 1);
-    mbar_init(&bar->drain, 1);
+    mbar_init(&bar->q_empty, 2);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bar->raw_full[s], 1);
       mbar_init(&bar->raw_empty[s], 4);
       mbar_init(&bar->k_full[s], 128);
-      mbar_init(&bar->k_empty[s], 1);
+      mbar_init(&bar->k_empty[s], 2);
       mbar_init(&bar->v_full[s], 128);
-      mbar_init(&bar->v_empty[s], 1);
+      mbar_init(&bar->v_empty[s], 2);
+      mbar_init(&bar->drain[s], 1);
       mbar_init(&bar->s_full[s], 1);
-      mbar_init(&bar->p_full[s], 128);
+      mbar_init(&bar->p_full[s][0], 256);
+      mbar_init(&bar->p_full[s][1], 256);
       mbar_init(&bar->o_done[s], 1);
-      mbar_init(&bar->o_free[s], 128);
+      mbar_init(&bar->o_free[s], 256);
     }
     fence_barrier_init();
     prefetch_tmap(&tmQ);
     prefetch_tmap(&tmK);
     prefetch_tmap(&tmV);
   }
-  if (warp == 13) {
+  if (warp == 21) {
     tmem_alloc(&bar->tmem, 512);
     tmem_relinquish();
   }
   pdl_trigger();
   pdl_wait();
-  // Tiles of each sequence (a warp each), then their sums.
+  // Steps of each sequence (a warp each), then their sums.  A CTA's share can end within an
+  // item's leading steps: it then has no tile of it (t0 == t1), and nothing behind it either.
   for (int b = warp; b < p.a.n_seq; b += kTcThreads / 32) {
     TcItem it;
     tc_sequence(p, b, it);
-    const int nb = (it.n_tok + 2 * p.tq - 1) / (2 * p.tq);
     int sum = 0;
-    for (int qb = lane; qb < nb; qb += 32) sum += tc_tiles(p, it.len, it.n_tok, qb);
+    for (int qb = lane; qb < it.nb; qb += 32) sum += kTcItemCost + tc_tiles(p, it.len, it.n_tok, qb);
     sum = __reduce_add_sync(0xffffffffu, sum);
     if (lane == 0) s_pre[b] = sum * c.heads;
   }
@@ -358,7 +377,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     set_max_regs_dec<kRegsWiden>();
     int n = 0;
     bool ok = true;
-    for (int x = lo; x < hi && ok;) {
+    for (int x = lo; x < hi && ok && it.t0 < it.t1;) {
       for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
 #pragma unroll 1
         for (int kv = 0; kv < 2; ++kv) {
@@ -390,7 +409,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
           const float4* con = s_const + (n & 3) * 8;
-          if (E4M3 && kv && ((t + 1) * kTcKeys > it.len || con[0].w != 2.0f)) {
+          if (E4M3 && ((t + 1) * kTcKeys > it.len || con[0].w != 2.0f)) {
             // Bytes that are no sequence's may be NaN, which a weight of 0 would not silence.
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
@@ -417,108 +436,167 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (lane == 0) mbar_arrive(&bar->raw_empty[kv]);
         }
       }
-      x += it.t1 - it.t0;
+      x = tc_end(it);
       if (x < hi) tc_next(p, it, x, hi);
     }
-  } else if (warp < 12) {
+  } else if (warp < 20) {
     // -------------------------------------------------------------- softmax
     set_max_regs_inc<kRegsSoftmax>();
-    const int side = (warp - 4) >> 2;
-    const int r = (warp & 3) * 32 + lane;  // row of the side's tile, TMEM lane
-    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + lane_base + side * 128;
-    const uint32_t tO = tmem + lane_base + Cfg::kColO + side * D;
+    const int side = (warp - 4) >> 3;
+    const int r0 = (warp & 3) * 32 + ((warp - 4) >> 2 & 1) * 16;  // the warp's first row of the side's tile
+    const int g = lane >> 2, t4 = lane & 3;
+    const uint32_t tS = tmem + (static_cast<uint32_t>(r0) << 16) + side * 128;
+    const uint32_t tO = tmem + (static_cast<uint32_t>(r0) << 16) + Cfg::kColO + side * D;
     int n = 0;
     bool ok = true;
-    for (int x = lo; x < hi && ok;) {
-      const int tok = (it.qb * 2 + side) * p.tq + r / p.a.group;
-      const bool row = r < p.tq * p.a.group && tok < it.n_tok;
-      const int lim = row && p.a.causal ? it.len - it.n_tok + tok + 1 : it.len;
-      float m = -INFINITY, l = 0.0f;
+    // Token within the side's, or far past any, and head within the group of the thread's rows.
+    int q_tok[2], q_head[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int q = r0 + g + 8 * r;
+      q_tok[r] = q < p.tq * p.a.group ? q / p.a.group : 0x40000000;
+      q_head[r] = q % p.a.group;
+    }
+    for (int x = lo; x < hi && ok && it.t0 < it.t1;) {
+      const int left = it.n_tok - (it.qb * 2 + side) * p.tq;  // tokens of the sequence from the side's first on
+      int lim[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        lim[r] = p.a.causal && q_tok[r] < left ? it.len - left + q_tok[r] + 1 : it.len;
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
       for (int t = it.t0; t < it.t1; ++t, ++n) {
+        const float4* con = s_const + (n & 3) * 8;
+        const int key = t * kTcKeys + 2 * t4;
         ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->s_full[side], n & 1, limit, c.err));
         if (!ok) break;
         tc_fence_after();
-        const float4* con = s_const + (n & 3) * 8;
-        const int k0 = t * kTcKeys;
-        const bool clean = __all_sync(0xffffffffu, k0 + kTcKeys <= lim && con[0].w == 2.0f);
-        const float mt = clean ? tc_row_max<false>(tS, con, k0, lim) : tc_row_max<true>(tS, con, k0, lim);
-        // Lazy rescaling: the row keeps its reference until the maximum passes it by 2^8.
-        const bool first = m == -INFINITY;
-        const bool rescale = !first && mt > m + kTcRescale;
-        const float m_new = first || rescale ? fmaxf(m, mt) : m;
-        const float base = m_new == -INFINITY ? 0.0f : m_new;
-        const float alpha = first ? 1.0f : ex2_approx(m - base);
-        if (__any_sync(0xffffffffu, rescale)) {
-          // P V of the tile before is complete: s_full was committed behind it.
-#pragma unroll 1
-          for (int i = 0; i < D / 32; ++i) {
-            uint32_t ov[32];
-            tmem_ld_32x32b_x32(tO + i * 32, ov);
-            tmem_wait_ld();
+        const bool clean =
+            __all_sync(0xffffffffu, (t + 1) * kTcKeys <= min(lim[0], lim[1]) && con[0].w == 2.0f);
+        float mt[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
-            tmem_st_32x32b_x32(tO + i * 32, ov);
+        for (int half = 0; half < 2; ++half) {
+          uint32_t v[32];
+          tc_half_load<KG>(tS + half * 64, con + half * 4, key + half * 64, lim, clean, v);
+          tc_half_max<KG>(v, con + half * 4, clean, mt);
+        }
+        // The rows keep their references until a maximum passes them by 2^14; only then do
+        // the four threads of a row compare theirs, and O is rescaled.
+        if (__any_sync(0xffffffffu, mt[0] > m[0] + kTcRescale || mt[1] > m[1] + kTcRescale)) {
+          float alpha[2];
+          bool rescale = false;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float u = fmaxf(mt[r], __shfl_xor_sync(0xffffffffu, mt[r], 1));
+            u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 2));
+            const bool grow = u > m[r] + kTcRescale;
+            alpha[r] = grow && m[r] != -INFINITY ? ex2_approx(m[r] - u) : 1.0f;
+            rescale |= alpha[r] != 1.0f;
+            m[r] = grow ? u : m[r];
+            l[r] *= alpha[r];
+          }
+          if (__any_sync(0xffffffffu, rescale)) {
+            // P V of the tile before is complete: s_full was committed behind it.
+#pragma unroll 1
+            for (int i = 0; i < D / 32; ++i) {
+              uint32_t ov[16];
+              tmem_ld_16x256b_x4(tO + i * 32, ov);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha[(e >> 1) & 1]);
+              tmem_st_16x256b_x4(tO + i * 32, ov);
+            }
           }
         }
-        m = m_new;
-        const float ls = clean ? tc_row_weights<false>(tS, con, k0, lim, base)
-                               : tc_row_weights<true>(tS, con, k0, lim, base);
-        l = fmaf(l, alpha, ls);
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&bar->p_full[side]);
+        // The sides' exponentials take turns: A after B's last tile, B after A's this one.  In
+        // step, both would want them at once and both would then want the tensor cores.
+        if (side == 1 || n > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->p_full[side ^ 1][1], side ? n & 1 : (n - 1) & 1,
+                                                        limit, c.err));
+          if (!ok) break;
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t v[32], pk[16];
+          tc_half_load<KG>(tS + half * 64, con + half * 4, key + half * 64, lim, clean, v);
+          tc_half_weights<KG>(v, con + half * 4, clean, m, l, pk);
+          __syncwarp();
+          tmem_st_16x128b_x8(tS + half * 32, pk);  // over columns that have been read
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&bar->p_full[side][half]);
+        }
       }
       if (!ok) break;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      }
       ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->o_done[side], (n - 1) & 1, limit, c.err));
       if (!ok) break;
       tc_fence_after();
       const bool whole = it.t1 - it.t0 == it.tiles;
-      const int64_t at = (it.first + tok) * p.a.n_heads + it.head * p.a.group + r % p.a.group;
-      const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + (it.t0 != 0 ? 0 : 1)) * kTcRows + side * 128 + r;
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      // A lane stores 8 columns of each 32: its row's four lanes trade theirs.
 #pragma unroll 1
       for (int i = 0; i < D / 32; ++i) {
-        uint32_t ov[32];
-        tmem_ld_32x32b_x32(tO + i * 32, ov);
+        uint32_t ov[16];
+        tmem_ld_16x256b_x4(tO + i * 32, ov);
         tmem_wait_ld();
-        if (row && whole) {
-          uint4* dst = reinterpret_cast<uint4*>(p.a.out + at * D + i * 32);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            __half2 h[4];
+        for (int r = 0; r < 2; ++r) {
+          const bool row = q_tok[r] < left;
+          const float inv = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
+          if (whole) {
+            uint32_t h[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              h[e] = __floats2half2_rn(__uint_as_float(ov[8 * q + 2 * e]) * inv,
-                                       __uint_as_float(ov[8 * q + 2 * e + 1]) * inv);
-            dst[q] = *reinterpret_cast<const uint4*>(h);
+            for (int j = 0; j < 4; ++j) {
+              const __half2 u = __floats2half2_rn(__uint_as_float(ov[4 * j + 2 * r]) * inv,
+                                                  __uint_as_float(ov[4 * j + 2 * r + 1]) * inv);
+              h[j] = *reinterpret_cast<const uint32_t*>(&u);
+            }
+            transpose4(h, t4);
+            const int64_t at = (it.first + it.n_tok - left + q_tok[r]) * p.a.n_heads + it.head * p.a.group + q_head[r];
+            if (row)
+              *reinterpret_cast<uint4*>(p.a.out + at * D + i * 32 + 8 * t4) = make_uint4(h[0], h[1], h[2], h[3]);
+            if (row && i == 0 && t4 == 0 && p.a.lse != nullptr)
+              p.a.lse[at] = l[r] == 0.0f ? -INFINITY : (m[r] + log2f(l[r])) * 0.69314718055994531f;
+          } else {
+            uint32_t f0[4], f1[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              f0[j] = ov[4 * j + 2 * r];
+              f1[j] = ov[4 * j + 2 * r + 1];
+            }
+            transpose4(f0, t4);
+            transpose4(f1, t4);
+            const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + (it.t0 != 0 ? 0 : 1)) * kTcRows +
+                                 side * 128 + r0 + g + 8 * r;
+            if (row) {
+              uint4* dst = reinterpret_cast<uint4*>(p.a.ws_o + part * D + i * 32 + 8 * t4);
+              dst[0] = make_uint4(f0[0], f1[0], f0[1], f1[1]);
+              dst[1] = make_uint4(f0[2], f1[2], f0[3], f1[3]);
+            }
+            if (row && i == 0 && t4 == 0) p.a.ws_ml[part] = make_float2(m[r], l[r]);
           }
-        } else if (row) {
-          uint4* dst = reinterpret_cast<uint4*>(p.a.ws_o + part * D + i * 32);
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            dst[q] = make_uint4(ov[4 * q], ov[4 * q + 1], ov[4 * q + 2], ov[4 * q + 3]);
         }
+        __syncwarp();
       }
-      if (row && whole && p.a.lse != nullptr)
-        p.a.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
-      if (row && !whole) p.a.ws_ml[part] = make_float2(m, l);
       tc_fence_before();
       mbar_arrive(&bar->o_free[side]);
-      x += it.t1 - it.t0;
+      x = tc_end(it);
       if (x < hi) tc_next(p, it, x, hi);
     }
   } else {
     set_max_regs_dec<kRegsOther>();
-    if (warp == 12) {
+    if (warp == 20) {
       // ----------------------------------------------------- lookups and TMA
       int n = 0, items = 0;
       bool ok = true;
       int4 cut = make_int4(-1, 0, 0, 0);
       const int per_box = min(4, 1 << (c.shift - 4));  // slices of 16 keys in a TMA box
-      for (int x = lo; x < hi && ok; ++items) {
+      for (int x = lo; x < hi && ok && it.t0 < it.t1; ++items) {
         if (it.t0 == 0 && it.t1 < it.tiles)
-          cut = make_int4(it.b, it.qb, it.head, (it.begin + it.tiles - 1) / per);
+          cut = make_int4(it.b, it.qb, it.head, (it.begin + kTcItemCost + it.tiles - 1) / per);
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->q_empty, (items & 1) ^ 1u, limit, c.err));
         if (!ok) break;
         if (lane == 0) {
@@ -571,7 +649,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           id = next;
         }
-        x += it.t1 - it.t0;
+        x = tc_end(it);
         if (x < hi) tc_next(p, it, x, hi);
       }
       if (lane == 0) p.a.cut[blockIdx.x] = cut;
@@ -582,88 +660,87 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         mbar_wait(&bar->raw_full[1], (n - 1) & 1, limit, c.err);
       }
       __syncwarp();
-    } else if (warp == 13 && lane == 0) {
-      // ----------------------------------------------------------------- MMA
+    } else if (warp == 21 || warp == 22) {
+      // ----------------------------------------------- MMA, a warp per side
+      // The whole warp walks the tiles and one lane issues; the operands' descriptors differ
+      // by constants only, so that an MMA costs an addition or two.
       constexpr uint32_t kIdescS = umma_idesc_f16(128, kTcKeys, false, false, false);
       constexpr uint32_t kIdescO = umma_idesc_f16(128, D, false, false, true);
+      const int side = warp - 21;
+      const bool leader = elect_one();
+      const uint64_t dq = umma_desc_sw128(smem_u32(smem + side * Cfg::kSide), 16, 1024);
+      const uint64_t dk = umma_desc_sw128(smem_u32(smem + Cfg::kOffK), 16, 1024);
+      const uint64_t dv = umma_desc_sw128(smem_u32(smem + Cfg::kOffV), 8192, 1024);
+      const uint32_t tS = tmem + side * 128, tO = tmem + Cfg::kColO + side * D;
       int n = 0, items = 0;
       bool ok = true;
       bool busy = false;  // something was issued
-      auto s_mma = [&](int side) {
-        const uint32_t qa = smem_u32(smem + side * Cfg::kSide);
-        const uint32_t ka = smem_u32(smem + Cfg::kOffK + (n & 1) * Cfg::kWide);
+      auto pv = [&](int i, bool start) {  // O += P V of tile i; `start`: the item's first
+        ok = mbar_wait(&bar->v_full[i & 1], (i >> 1) & 1, limit, c.err);
+        // It overwrites O: the last item's rows have been read.
+        if (ok && start) ok = mbar_wait(&bar->o_free[side], (items & 1) ^ 1u, limit, c.err);
+        const uint64_t d = dv + static_cast<uint64_t>((i & 1) * (Cfg::kWide >> 4));
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t ad = umma_desc_sw128(qa + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024);
-          const uint64_t bd = umma_desc_sw128(ka + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024);
-          umma_f16(tmem + side * 128, ad, bd, kIdescS, kk > 0 ? 1u : 0u);
-        }
-        umma_commit(&bar->s_full[side]);
-      };
-      auto pv_mma = [&](int side, int i, bool start) {  // O += P V of tile i
-        const uint32_t va = smem_u32(smem + Cfg::kOffV + (i & 1) * Cfg::kWide);
+        for (int half = 0; half < 2; ++half) {
+          if (ok) ok = mbar_wait(&bar->p_full[side][half], i & 1, limit, c.err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) return;
+          tc_fence_after();
+          if (leader) {
 #pragma unroll
-        for (int kk = 0; kk < kTcKeys / 16; ++kk) {
-          const uint64_t bd =
-              umma_desc_sw128(va + (kk >> 2) * (Cfg::kDH * 8192) + (kk & 3) * 2048, 8192, 1024);
-          umma_f16_ts(tmem + Cfg::kColO + side * D, tmem + side * 128 + kk * 8, bd, kIdescO,
-                      (start && kk == 0) ? 0u : 1u);
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f16_ts(tO, tS + half * 32 + kk * 8, d + ((half * (Cfg::kDH * 8192) + kk * 2048) >> 4), kIdescO,
+                          (start && half == 0 && kk == 0) ? 0u : 1u);
+            if (half == 1) {
+              umma_commit(&bar->o_done[side]);
+              umma_commit(&bar->v_empty[i & 1]);
+            }
+          }
+          __syncwarp();
+          busy = true;
         }
-        umma_commit(&bar->o_done[side]);
       };
-      for (int x = lo; x < hi && ok; ++items) {
+      for (int x = lo; x < hi && ok && it.t0 < it.t1; ++items) {
         ok = mbar_wait(&bar->q_full, items & 1, limit, c.err);
         for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
           ok = mbar_wait(&bar->k_full[n & 1], (n >> 1) & 1, limit, c.err);
-          if (ok && t > it.t0) ok = mbar_wait(&bar->v_full[(n - 1) & 1], ((n - 1) >> 1) & 1, limit, c.err);
-          for (int side = 0; side < 2 && ok; ++side) {
-            if (t > it.t0) {
-              ok = mbar_wait(&bar->p_full[side], (n - 1) & 1, limit, c.err);
-              // The first product of an item overwrites O: the last item's rows have been read.
-              if (ok && t == it.t0 + 1) ok = mbar_wait(&bar->o_free[side], (items & 1) ^ 1u, limit, c.err);
-              if (!ok) break;
-              tc_fence_after();
-              pv_mma(side, n - 1, t == it.t0 + 1);
-              busy = true;
-              if (side == 1) umma_commit(&bar->v_empty[(n - 1) & 1]);
-            }
-            // S goes over P of the tile before: its product must have read it.
-            if (n > 0) ok = mbar_wait(&bar->o_done[side], (n - 1) & 1, limit, c.err);
-            if (!ok) break;
-            tc_fence_after();
-            s_mma(side);
-            busy = true;
-          }
-          if (ok) umma_commit(&bar->k_empty[n & 1]);
-        }
-        if (!ok) break;
-        umma_commit(&bar->q_empty);
-        // The item's last tile.
-        const bool start = it.t1 - it.t0 == 1;
-        ok = mbar_wait(&bar->v_full[(n - 1) & 1], ((n - 1) >> 1) & 1, limit, c.err);
-        for (int side = 0; side < 2 && ok; ++side) {
-          ok = mbar_wait(&bar->p_full[side], (n - 1) & 1, limit, c.err);
-          if (ok && start) ok = mbar_wait(&bar->o_free[side], (items & 1) ^ 1u, limit, c.err);
+          if (ok && t > it.t0) pv(n - 1, t == it.t0 + 1);
+          // S goes over P of the tile before: its product must have read it.
+          if (ok && n > 0) ok = mbar_wait(&bar->o_done[side], (n - 1) & 1, limit, c.err);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
-          pv_mma(side, n - 1, start);
+          if (leader) {
+            const uint64_t d = dk + static_cast<uint64_t>((n & 1) * (Cfg::kWide >> 4));
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              umma_f16(tS, dq + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
+                       d + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), kIdescS, kk > 0 ? 1u : 0u);
+            umma_commit(&bar->s_full[side]);
+            umma_commit(&bar->k_empty[n & 1]);
+          }
+          __syncwarp();
           busy = true;
         }
-        if (ok) umma_commit(&bar->v_empty[(n - 1) & 1]);
-        x += it.t1 - it.t0;
+        if (!ok) break;
+        if (leader) umma_commit(&bar->q_empty);
+        __syncwarp();
+        pv(n - 1, it.t1 - it.t0 == 1);
+        x = tc_end(it);
         if (x < hi) tc_next(p, it, x, hi);
       }
       // No MMA may still use TMEM or shared memory when the CTA leaves.
       if (busy) {
-        umma_commit(&bar->drain);
-        mbar_wait(&bar->drain, 0, limit, c.err);
+        if (leader) umma_commit(&bar->drain[side]);
+        __syncwarp();
+        mbar_wait(&bar->drain[side], 0, limit, c.err);
       }
     }
     __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 13) {
+  if (warp == 21) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -709,10 +786,10 @@ __global__ void __launch_bounds__(2 * D) attn_paged_tc_join_kernel(const TcParam
     p.a.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
-template <int D, bool E4M3>
-int launch_tc(TcParams p, const engine_kv_pages_t* kv, int64_t most_tiles, cudaStream_t st) {
+template <int D, bool E4M3, int KG>
+int launch_tc(TcParams p, const engine_kv_pages_t* kv, int64_t most_steps, cudaStream_t st) {
   using Cfg = TcCfg<D>;
-  auto kern = attn_paged_tc_kernel<D, E4M3>;
+  auto kern = attn_paged_tc_kernel<D, E4M3, KG>;
   static std::atomic<uint64_t> configured{0};
   int dev = 0;
   B200_CUDA(cudaGetDevice(&dev));
@@ -732,7 +809,7 @@ int launch_tc(TcParams p, const engine_kv_pages_t* kv, int64_t most_tiles, cudaS
   const uint64_t strides[2] = {static_cast<uint64_t>(D), static_cast<uint64_t>(p.a.q_pitch)};
   const uint32_t qbox[3] = {64, static_cast<uint32_t>(p.a.group), static_cast<uint32_t>(p.tq)};
   if (!make_tmap_3d(&tq, p.a.q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, dims, strides, qbox)) return ENGINE_ERR_CUDA;
-  const int64_t ctas = std::min<int64_t>(sm_count(), most_tiles);
+  const int64_t ctas = std::min<int64_t>(sm_count(), most_steps);
   const size_t o_bytes = 2 * ctas * kTcRows * D * sizeof(float), ml_bytes = 2 * ctas * kTcRows * sizeof(float2);
   char* ws = static_cast<char*>(scratch_alloc(o_bytes + ml_bytes + ctas * sizeof(int4), st));
   if (ws == nullptr)
@@ -755,15 +832,23 @@ int attention_paged_tc(const ApParams& a, const engine_kv_pages_t* kv, cudaStrea
   TcParams p;
   p.a = a;
   p.tq = 128 / a.group;
-  // At most this many tiles (the kernel counts them in 32 bits).
-  const int64_t tiles = std::max<int64_t>((kv->max_pages * kv->page_size + kTcKeys - 1) / kTcKeys, 1);
+  // At most this many steps (the kernel counts them in 32 bits).
+  const int64_t tiles = std::max<int64_t>((kv->max_pages * kv->page_size + kTcKeys - 1) / kTcKeys, 1) + kTcItemCost;
   const int64_t blocks = a.n_tokens / (2 * p.tq) + a.n_seq;
   if (blocks > 0x7fffffff / kv->n_kv_heads / tiles)
     return set_error(ENGINE_ERR_UNSUPPORTED, "attention_paged_prefill: too many query rows x positions");
   const int64_t most = blocks * kv->n_kv_heads * tiles;
-  const bool e4m3 = kv->type == ENGINE_KV_E4M3;
-  if (kv->head_dim == 64) return e4m3 ? launch_tc<64, true>(p, kv, most, st) : launch_tc<64, false>(p, kv, most, st);
-  return e4m3 ? launch_tc<128, true>(p, kv, most, st) : launch_tc<128, false>(p, kv, most, st);
+  // Keys that share constants within a half tile: the page's.
+  auto run = [&](auto kg) {
+    constexpr int KG = decltype(kg)::value;
+    const bool e4m3 = kv->type == ENGINE_KV_E4M3;
+    if (kv->head_dim == 64)
+      return e4m3 ? launch_tc<64, true, KG>(p, kv, most, st) : launch_tc<64, false, KG>(p, kv, most, st);
+    return e4m3 ? launch_tc<128, true, KG>(p, kv, most, st) : launch_tc<128, false, KG>(p, kv, most, st);
+  };
+  if (kv->page_size == 16) return run(std::integral_constant<int, 16>());
+  if (kv->page_size == 32) return run(std::integral_constant<int, 32>());
+  return run(std::integral_constant<int, 64>());
 }
 
 }  // namespace b200
