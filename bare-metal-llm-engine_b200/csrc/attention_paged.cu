@@ -46,19 +46,21 @@ constexpr int kPgThreads = (kPgConsumers + 1) * 32;
 constexpr int kPgMaxSeq = 1024;  // sequences per launch (their prefix sums sit in shared memory)
 constexpr float kPgRescale = 8.0f;
 constexpr int64_t kManyRows = 32;  // from here on attention_paged_tc
+constexpr int64_t kWholeTiles = 16;  // slots of at most so many tiles: a CTA to an item
 static_assert(kPgMaxSeq <= kTcMaxSeq, "both kernels take a launch's sequences");
 
-/// NQ: groups of 8 query rows of an item.  One: 3 CTAs an SM with 128 registers a
-/// thread; two need about 170: 2 CTAs.
+/// NQ: groups of 8 query rows of an item.  Three CTAs an SM with 128 registers a thread
+/// either way: of sixteen rows the fragments of q stay in shared memory.
 template <int D, int NQ>
 struct PgCfg {
   static constexpr int kRows = 8 * NQ;
-  static constexpr int kCtas = NQ == 1 ? 3 : 2;
+  static constexpr int kCtas = 3;
   static constexpr int kTile = kPgKeys * D;  // bytes of K (or V) of a tile
-  static constexpr int kStages = (NQ == 1 ? 4 : 6) * (D == 128 ? 2 : 3) / 2;
+  static constexpr int kStages = (NQ == 1 ? 4 : 3) * 128 / D * (D == 128 ? 4 : 3) / 4;
   static constexpr int kOW = D + 4;          // pitch of a row of O in shared memory
   static constexpr int kOffO = kStages * 2 * kTile;
-  static constexpr int kOffConst = kOffO + kRows * kOW * 4;
+  static constexpr int kOffQ = kOffO + kRows * kOW * 4;       // [D / 16][32 lanes], 16 bytes each
+  static constexpr int kOffConst = kOffQ + (NQ == 1 ? 0 : D / 16 * 512);
   static constexpr int kOffBar = kOffConst + kStages * 4 * 16;
   static constexpr int kOffMl = kOffBar + 2 * kStages * 8;
   static constexpr int kOffSeq = kOffMl + kPgConsumers * kRows * 8;
@@ -138,7 +140,7 @@ struct PgLists {
   const int32_t* len;
 };
 
-/// The item at tile `x`, up to tile `hi`.
+/// The item at tile `x` (`whole`: the item of that number), up to tile `hi`.
 __device__ __forceinline__ PgItem pg_item(const ApParams& p, const PgLists& s, int x, int hi) {
   int lo = 0, up = p.n_seq - 1;
   while (lo < up) {  // the last sequence that starts at or before x
@@ -152,9 +154,9 @@ __device__ __forceinline__ PgItem pg_item(const ApParams& p, const PgLists& s, i
   it.len = s.len[lo];
   it.tiles = max((it.len + kPgKeys - 1) / kPgKeys, 1);
   const int y = x - s.pre[lo];
-  const int j = y / it.tiles;
-  it.t0 = y - j * it.tiles;
-  it.t1 = min(it.tiles, it.t0 + hi - x);
+  const int j = p.whole ? y : y / it.tiles;
+  it.t0 = p.whole ? 0 : y - j * it.tiles;
+  it.t1 = p.whole ? it.tiles : min(it.tiles, it.t0 + hi - x);
   it.begin = x - it.t0;
   it.head = j % p.c.heads;
   it.row0 = j / p.c.heads * kPgRows;
@@ -179,6 +181,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   float* s_o = reinterpret_cast<float*>(smem + Cfg::kOffO);
+  uint4* s_q = reinterpret_cast<uint4*>(smem + Cfg::kOffQ);
   float4* s_const = reinterpret_cast<float4*>(smem + Cfg::kOffConst);  // [ST][4]: of 16 keys each
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
   uint64_t* empty = full + ST;
@@ -207,7 +210,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
     const int rows = kv_rows(p.c, p.cu, p.seq0 + b, p.n_tokens, &first) * p.group;
     s_slot[b] = slot;
     s_len[b] = len;
-    s_pre[b] = (rows + kPgRows - 1) / kPgRows * p.c.heads * max((len + kPgKeys - 1) / kPgKeys, 1);
+    s_pre[b] = (rows + kPgRows - 1) / kPgRows * p.c.heads * (p.whole ? 1 : max((len + kPgKeys - 1) / kPgKeys, 1));
   }
   __syncthreads();
   if (warp == 0) {
@@ -228,6 +231,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
   __syncthreads();
   const PgLists lists{s_pre, s_slot, s_len};
   const int total = s_pre[p.n_seq];
+  // Tiles (items, where `whole`) to a CTA.
   const int per = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
   const int lo = min(static_cast<int64_t>(blockIdx.x) * per, static_cast<int64_t>(total));
   const int hi = min(lo + per, total);
@@ -235,11 +239,12 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
   if (warp == kPgConsumers) {
     // ------------------------------------------------------------ producer
     const float kc_unit = p.scale_log2 * (E4M3 ? 1.0f : 1.0f / kKeyUnit);
-    int n = 0;  // tiles issued
+    int n = 0, issued = 0;  // tiles handed over, and fetched
+    int page_base = 0;
     bool ok = true;
     for (int x = lo; x < hi && ok;) {
       const PgItem it = pg_item(p, lists, x, hi);
-      x += it.t1 - it.t0;
+      x += p.whole ? 1 : it.t1 - it.t0;
       const int n_keys = it.len;
       const int first_slice = it.t0 * 4, end_slice = min(it.t1 * 4, (n_keys + 15) >> 4);
       // Lane i of batch k looks after slice first_slice + 32 k + i.
@@ -252,7 +257,35 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
         ks = p.c.ks[kv_scale_at(p.c, id, it.head)];
         vs = p.c.vs[kv_scale_at(p.c, id, it.head)];
       }
+      // One load per page of a tile, by the lane of the page's first slice.
+      const int per_box = p.c.shift >= 6 ? 4 : 1 << (p.c.shift - 4);
+      auto fetch = [&](int at, int i) {  // tile number `at`, the batch's i-th
+        const int s = at % ST;
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((at / ST) & 1u) ^ 1u, p.limit_ns, p.c.err));
+        if (!ok) return;
+        const int slice = lane & 3;
+        const bool mine = (lane >> 2) == i && id >= 0 && slice % per_box == 0;
+        const unsigned who = __ballot_sync(0xffffffffu, mine);
+        if (lane == 0) mbar_expect_tx(&full[s], __popc(who) * per_box * 16 * D * 2);
+        __syncwarp();
+        if (mine) {
+          uint8_t* sk = smem + s * 2 * Cfg::kTile + slice * 16 * D;
+          const int key = (first_slice + lane) * 16 + page_base;
+          const int off = key & ((1 << p.c.shift) - 1);  // row within the page
+          const int row = ((id * p.c.heads + it.head) << p.c.shift) + off;
+          const int y = D == 128 ? row : row >> 1;
+          tma_load_2d(sk, &tmK, &full[s], 0, y);
+          tma_load_2d(sk + Cfg::kTile, &tmV, &full[s], 0, y);
+        }
+      };
       for (int base = it.t0; base < it.t1 && ok; base += 8) {
+        page_base = (base - it.t0) * kPgKeys;
+        const int count = min(8, it.t1 - base);
+        // At the CTA's start the first tiles are on their way before the scales are here.
+        int ahead = 0;
+        if (n == 0) {
+          for (; ahead < min(count, ST) && ok; ++ahead) fetch(ahead, ahead);
+        }
         const int id2 = page_of((base + 16) * 4 + lane);
         if (id1 >= 0) {
           ks1 = p.c.ks[kv_scale_at(p.c, id1, it.head)];
@@ -261,32 +294,15 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
         const float v1 = vs == 0.0f ? 1.0f : vs;
         const float4 con = id >= 0 ? make_float4(ks * kc_unit, log2f(v1), 1.0f / v1, 1.0f)
                                    : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
-        for (int i = 0; i < 8 && base + i < it.t1; ++i, ++n) {
-          const int s = n % ST;
-          ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((n / ST) & 1u) ^ 1u, p.limit_ns, p.c.err));
+        for (int i = 0; i < count && ok; ++i, ++n) {
+          if (i >= ahead) fetch(n, i);
           if (!ok) break;
+          const int s = n % ST;
           if (lane >> 2 == i) s_const[s * 4 + (lane & 3)] = con;
           __syncwarp();
-          // One load per page of the tile: by the lane of the page's first slice.
-          const int slice = lane & 3;
-          const int per_page = p.c.shift >= 6 ? 4 : 1 << (p.c.shift - 4);
-          const bool mine = (lane >> 2) == i && id >= 0 && slice % per_page == 0;
-          const unsigned who = __ballot_sync(0xffffffffu, mine);
-          if (lane == 0) {
-            const uint32_t bytes = __popc(who) * per_page * 16 * D * 2;
-            mbar_arrive_expect_tx(&full[s], bytes);
-          }
-          __syncwarp();
-          if (mine) {
-            uint8_t* sk = smem + s * 2 * Cfg::kTile + slice * 16 * D;
-            const int key = (base + i) * kPgKeys + slice * 16;
-            const int off = key & ((1 << p.c.shift) - 1);  // row within the page
-            const int row = ((id * p.c.heads + it.head) << p.c.shift) + off;
-            const int y = D == 128 ? row : row >> 1;
-            tma_load_2d(sk, &tmK, &full[s], 0, y);
-            tma_load_2d(sk + Cfg::kTile, &tmV, &full[s], 0, y);
-          }
+          if (lane == 0) mbar_arrive(&full[s]);
         }
+        issued = max(n, ahead);
         id = id1;
         ks = ks1;
         vs = vs1;
@@ -294,6 +310,13 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
       }
     }
     // No copy may still be writing shared memory when the CTA leaves.
+    // (Behind a wait that ran out, tiles that were fetched ahead have not been arrived for.)
+    if (n < issued) {
+      for (; n < issued; ++n) {
+        if (lane == 0) mbar_arrive(&full[n % ST]);
+        __syncwarp();
+      }
+    }
     for (int j = max(n - ST, 0); j < n; ++j) mbar_wait(&full[j % ST], (j / ST) & 1u, p.limit_ns, p.c.err);
   } else {
     // ----------------------------------------------------------- consumers
@@ -301,13 +324,13 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
     constexpr int NK = D / 16;  // contraction steps of S^T, and 16-row tiles of O^T
     int n = 0;
     bool ok = true;
-    if (threadIdx.x == 0) p.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (threadIdx.x == 0 && !p.whole) p.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
     for (int x = lo; x < hi;) {
       const PgItem it = pg_item(p, lists, x, hi);
-      x += it.t1 - it.t0;
+      x += p.whole ? 1 : it.t1 - it.t0;
       // q^T as B fragments: the lane's D / 4 elements of query row g (and g + 8), from
       // t * D / 4.  In the sums' columns a lane has rows 2t and 2t + 1 (and + 8).
-      uint32_t bq[NQ][NK][2];
+      uint32_t bq[NQ == 1 ? NK : 1][2];
       float init[NQ][2];
       int lim[NQ][2];
       int least = it.len;
@@ -325,16 +348,20 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
           const uint32_t q[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const uint32_t u0 = q[2 * e], u1 = q[2 * e + 1];
-            if constexpr (E4M3) {
-              bq[nq][2 * i + e][0] = u0;
-              bq[nq][2 * i + e][1] = u1;
-            } else {  // elements (0, 2) and (1, 3), as k_fragment pairs the codes
-              bq[nq][2 * i + e][0] = __byte_perm(u0, u1, 0x5410);
-              bq[nq][2 * i + e][1] = __byte_perm(u0, u1, 0x7632);
+            uint32_t u0 = q[2 * e], u1 = q[2 * e + 1];
+            if constexpr (!E4M3) {  // elements (0, 2) and (1, 3), as k_fragment pairs the codes
               const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&u0));
               const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&u1));
               sum += (f0.x + f0.y) + (f1.x + f1.y);
+              const uint32_t v0 = u0;
+              u0 = __byte_perm(v0, u1, 0x5410);
+              u1 = __byte_perm(v0, u1, 0x7632);
+            }
+            if constexpr (NQ == 1) {
+              bq[2 * i + e][0] = u0;
+              bq[2 * i + e][1] = u1;
+            } else if (warp == 0) {
+              reinterpret_cast<uint2*>(s_q + (2 * i + e) * 32 + lane)[nq] = make_uint2(u0, u1);
             }
           }
         }
@@ -350,6 +377,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
         }
       }
       least = __reduce_min_sync(0xffffffffu, least);
+      if (NQ > 1) consumer_sync();  // s_q
       float o[NQ][NK][4];
       float m[NQ][2], l[NQ][2];
 #pragma unroll
@@ -389,8 +417,13 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
           uint32_t a[4];
           k_fragment<E4M3>(kw[0][i], a[0], a[2]);
           k_fragment<E4M3>(kw[1][i], a[1], a[3]);
-#pragma unroll
-          for (int nq = 0; nq < NQ; ++nq) mma16816(sc[nq], a, bq[nq][i][0], bq[nq][i][1]);
+          if constexpr (NQ == 1) {
+            mma16816(sc[0], a, bq[i][0], bq[i][1]);
+          } else {
+            const uint4 b = s_q[i * 32 + lane];
+            mma16816(sc[0], a, b.x, b.y);
+            mma16816(sc[NQ - 1], a, b.z, b.w);
+          }
         }
         // The lane's D / 8 elements, from g * D / 8, of keys 2t, 2t+1, 2t+8, 2t+9: on their way
         // while the weights are formed.
@@ -575,21 +608,26 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
       }
       if (threadIdx.x == 0 && it.t0 == 0 && !whole)
         p.cut[blockIdx.x] = make_int4(it.b, it.row0, it.head, (it.begin + it.tiles - 1) / per);
-      consumer_sync();  // s_o and s_ml are free again
+      consumer_sync();  // s_o, s_ml and s_q are free again
     }
   }
 }
 
 /// Joins the parts of the item that CTA blockIdx.x of attn_paged_kernel began and did
 /// not finish (its part 1, and part 0 of each CTA up to the one that finished it);
-/// blockIdx.y is the row, thread i has column i.
+/// blockIdx.y is the row.  One sequence of 131072 keys has 55 parts of a row: eight warps
+/// take every eighth, so that all of them are on their way at once.
+constexpr int kJoinWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(D) attn_paged_join_kernel(const ApParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const ApParams p) {
   pdl_trigger();
   pdl_wait();
   const int4 cut = p.cut[blockIdx.x];
   if (cut.x < 0) return;
-  const int row = blockIdx.y, col = threadIdx.x;
+  constexpr int E = D / 32;  // columns of a lane
+  __shared__ float s_o[kJoinWarps][D];
+  __shared__ float s_l[kJoinWarps];
+  const int row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int64_t first;
   const int n_rows = kv_rows(p.c, p.cu, p.seq0 + cut.x, p.n_tokens, &first) * p.group;
   if (cut.y + row >= n_rows) return;
@@ -597,26 +635,45 @@ __global__ void __launch_bounds__(D) attn_paged_join_kernel(const ApParams p) {
   const int part0 = 2 * static_cast<int>(blockIdx.x);
   auto slot = [&](int i) { return static_cast<int64_t>(part0 + (i == 0 ? 1 : 2 * i)) * kPgRows + row; };
   float m = -INFINITY;
+  for (int i = lane; i < parts; i += 32) m = fmaxf(m, p.ws_ml[slot(i)].x);
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+  float l = 0.0f, o[E] = {};
 #pragma unroll 4
-  for (int i = 0; i < parts; ++i) m = fmaxf(m, p.ws_ml[slot(i)].x);
-  float l = 0.0f, o = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
+  for (int i = warp; i < parts; i += kJoinWarps) {
     const float2 ml = p.ws_ml[slot(i)];
+    float v[E];
+    if constexpr (E == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p.ws_o + slot(i) * D + lane * E);
+    else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(p.ws_o + slot(i) * D + lane * E);
     // A part without a visible key has m = -inf, l = 0 and o = 0 (or NaN in all: kept).
     const float a = ml.x == -INFINITY ? 1.0f : ex2_approx(ml.x - m);
     l = fmaf(ml.y, a, l);
-    o = fmaf(p.ws_o[slot(i) * D + col], a, o);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(v[e], a, o[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
+  if (lane == 0) s_l[warp] = l;
+  __syncthreads();
+  const int col = threadIdx.x;
+  if (col >= D) return;
+  float sum = 0.0f;
+  l = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    sum += s_o[w][col];
+    l += s_l[w];
   }
   const int64_t at = pg_row(p, first, cut.z, cut.y + row);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  p.out[at * D + col] = __float2half_rn(o * inv);
+  p.out[at * D + col] = __float2half_rn(sum * inv);
   if (p.lse != nullptr && col == 0)
     p.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
+/// `most`: tiles (items, where p.whole) that there can be.
 template <int D, bool E4M3, int NQ>
-int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most_tiles, cudaStream_t st) {
+int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most, cudaStream_t st) {
   using Cfg = PgCfg<D, NQ>;
   auto kern = attn_paged_kernel<D, E4M3, NQ>;
   const size_t smem = Cfg::smem(p.n_seq);
@@ -637,7 +694,12 @@ int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most_tiles, cu
     return ENGINE_ERR_CUDA;
   // kCtas an SM while their shared memory fits (three: up to about 300 sequences).
   const int64_t per_sm = std::min<int64_t>(Cfg::kCtas, (max_smem_optin() + 1024) / static_cast<int64_t>(smem + 1024));
-  const int64_t ctas = std::min<int64_t>(sm_count() * std::max<int64_t>(per_sm, 1), most_tiles);
+  if (p.whole) {
+    const cudaError_t e =
+        launch_pdl(kern, dim3(static_cast<unsigned>(most)), dim3(kPgThreads), smem, st, tk, tv, p);
+    return e == cudaSuccess ? ENGINE_OK : set_cuda_error(e, "attn_paged_kernel");
+  }
+  const int64_t ctas = std::min<int64_t>(sm_count() * std::max<int64_t>(per_sm, 1), most);
   const size_t o_bytes = 2 * ctas * kPgRows * D * sizeof(float), ml_bytes = 2 * ctas * kPgRows * sizeof(float2);
   char* ws = static_cast<char*>(scratch_alloc(o_bytes + ml_bytes + ctas * sizeof(int4), st));
   if (ws == nullptr) return set_error(ENGINE_ERR_CUDA, "attention_paged: workspace allocation failed");
@@ -647,7 +709,8 @@ int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most_tiles, cu
   int rc = ENGINE_OK;
   cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPgThreads), smem, st, tk, tv, p);
   if (e == cudaSuccess)
-    e = launch_pdl(attn_paged_join_kernel<D>, dim3(static_cast<unsigned>(ctas), Cfg::kRows), dim3(D), 0, st, p);
+    e = launch_pdl(attn_paged_join_kernel<D>, dim3(static_cast<unsigned>(ctas), Cfg::kRows), dim3(kJoinWarps * 32), 0,
+                   st, p);
   if (e != cudaSuccess) rc = set_cuda_error(e, "attn_paged_kernel");
   scratch_free(ws, st);
   return rc;
@@ -673,7 +736,8 @@ int run_paged(ApParams p, const engine_kv_pages_t* kv, int64_t n_seq, cudaStream
                                            : p.n_tokens * p.group / kPgRows + n;
     if (groups > 0x7fffffff / kv->n_kv_heads / tiles)
       return set_error(ENGINE_ERR_UNSUPPORTED, std::string(what) + ": too many query rows x positions");
-    const int64_t most = groups * kv->n_kv_heads * tiles;
+    p.whole = tiles <= kWholeTiles ? 1 : 0;
+    const int64_t most = groups * kv->n_kv_heads * (p.whole ? 1 : tiles);
     int rc;
     if (kv->head_dim == 64) {
       rc = e4m3 ? (r8 ? launch_paged<64, true, 1>(p, kv, most, st) : launch_paged<64, true, 2>(p, kv, most, st))

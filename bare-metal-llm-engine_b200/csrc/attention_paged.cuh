@@ -23,6 +23,7 @@ struct ApParams {
   float* ws_o;        // [2 * CTAs][rows][D]: unfinished items, part 1 of the CTA that began one,
   float2* ws_ml;      // [2 * CTAs][rows]     part 0 of those that went on with it
   int4* cut;          // [CTAs]: the item that a CTA began and did not finish
+  int whole;          // a CTA to an item: none is cut, no workspace
   unsigned long long limit_ns;
 };
 
