@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
     constexpr int NK = D / 16;  // contraction steps of S^T, and 16-row tiles of O^T
     int n = 0;
     bool ok = true;
-    if (threadIdx.x == 0 && !p.whole) p.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (threadIdx.x == 0 && !p.whole && !p.by_item) p.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
     for (int x = lo; x < hi;) {
       const PgItem it = pg_item(p, lists, x, hi);
       x += p.whole ? 1 : it.t1 - it.t0;
@@ -606,16 +606,19 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
           if (col == 0) p.ws_ml[wslot * kPgRows + row] = make_float2(mm, ll);
         }
       }
-      if (threadIdx.x == 0 && it.t0 == 0 && !whole)
-        p.cut[blockIdx.x] = make_int4(it.b, it.row0, it.head, (it.begin + it.tiles - 1) / per);
+      if (threadIdx.x == 0 && it.t0 == 0 && !p.whole && (p.by_item || !whole)) {
+        const int parts = (it.begin + it.tiles - 1) / per - static_cast<int>(blockIdx.x) + 1;
+        const int at = p.by_item ? (it.b * ((p.group + kPgRows - 1) / kPgRows) + it.row0 / kPgRows) * p.c.heads + it.head
+                                 : static_cast<int>(blockIdx.x);
+        p.cut[at] = make_int4(whole ? -1 : it.b, it.row0, it.head | parts << 16, static_cast<int>(blockIdx.x));
+      }
       consumer_sync();  // s_o, s_ml and s_q are free again
     }
   }
 }
 
-/// Joins the parts of the item that CTA blockIdx.x of attn_paged_kernel began and did
-/// not finish (its part 1, and part 0 of each CTA up to the one that finished it);
-/// blockIdx.y is the row.  One sequence of 131072 keys has 55 parts of a row: eight warps
+/// Joins the parts of a cut item (part 1 of the CTA that began it, and part 0 of each one
+/// up to that which finished it); blockIdx.x is the entry of p.cut, blockIdx.y the row.  One sequence of 131072 keys has 55 parts of a row: eight warps
 /// take every eighth, so that all of them are on their way at once.
 constexpr int kJoinWarps = 8;
 template <int D>
@@ -631,8 +634,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
   int64_t first;
   const int n_rows = kv_rows(p.c, p.cu, p.seq0 + cut.x, p.n_tokens, &first) * p.group;
   if (cut.y + row >= n_rows) return;
-  const int parts = cut.w - static_cast<int>(blockIdx.x) + 1;
-  const int part0 = 2 * static_cast<int>(blockIdx.x);
+  const int parts = static_cast<int>(static_cast<unsigned>(cut.z) >> 16);
+  const int part0 = 2 * cut.w;
   auto slot = [&](int i) { return static_cast<int64_t>(part0 + (i == 0 ? 1 : 2 * i)) * kPgRows + row; };
   float m = -INFINITY;
   for (int i = lane; i < parts; i += 32) m = fmaxf(m, p.ws_ml[slot(i)].x);
@@ -664,7 +667,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
     sum += s_o[w][col];
     l += s_l[w];
   }
-  const int64_t at = pg_row(p, first, cut.z, cut.y + row);
+  const int64_t at = pg_row(p, first, cut.z & 0xffff, cut.y + row);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   p.out[at * D + col] = __float2half_rn(sum * inv);
   if (p.lse != nullptr && col == 0)
@@ -700,8 +703,13 @@ int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most, cudaStre
     return e == cudaSuccess ? ENGINE_OK : set_cuda_error(e, "attn_paged_kernel");
   }
   const int64_t ctas = std::min<int64_t>(sm_count() * std::max<int64_t>(per_sm, 1), most);
+  // One row per sequence: the items are numbered, and the join has a block column for each.
+  // Else they are known by the CTA that began them.
+  const int64_t items = static_cast<int64_t>(p.n_seq) * ((p.group + kPgRows - 1) / kPgRows) * p.c.heads;
+  p.by_item = p.cu == nullptr && items <= ctas ? 1 : 0;
+  const int64_t cuts = p.by_item ? items : ctas;
   const size_t o_bytes = 2 * ctas * kPgRows * D * sizeof(float), ml_bytes = 2 * ctas * kPgRows * sizeof(float2);
-  char* ws = static_cast<char*>(scratch_alloc(o_bytes + ml_bytes + ctas * sizeof(int4), st));
+  char* ws = static_cast<char*>(scratch_alloc(o_bytes + ml_bytes + cuts * sizeof(int4), st));
   if (ws == nullptr) return set_error(ENGINE_ERR_CUDA, "attention_paged: workspace allocation failed");
   p.ws_o = reinterpret_cast<float*>(ws);
   p.ws_ml = reinterpret_cast<float2*>(ws + o_bytes);
@@ -709,7 +717,7 @@ int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most, cudaStre
   int rc = ENGINE_OK;
   cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPgThreads), smem, st, tk, tv, p);
   if (e == cudaSuccess)
-    e = launch_pdl(attn_paged_join_kernel<D>, dim3(static_cast<unsigned>(ctas), Cfg::kRows), dim3(kJoinWarps * 32), 0,
+    e = launch_pdl(attn_paged_join_kernel<D>, dim3(static_cast<unsigned>(cuts), Cfg::kRows), dim3(kJoinWarps * 32), 0,
                    st, p);
   if (e != cudaSuccess) rc = set_cuda_error(e, "attn_paged_kernel");
   scratch_free(ws, st);

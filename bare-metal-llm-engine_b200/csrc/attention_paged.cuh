@@ -22,7 +22,9 @@ struct ApParams {
   float scale_log2;
   float* ws_o;        // [2 * CTAs][rows][D]: unfinished items, part 1 of the CTA that began one,
   float2* ws_ml;      // [2 * CTAs][rows]     part 0 of those that went on with it
-  int4* cut;          // [CTAs]: the item that a CTA began and did not finish
+  int4* cut;          // items that are cut: sequence (-1: none), first row, KV head (16-row
+                      // kernel: and parts << 16), last CTA (16-row kernel: the first)
+  int by_item;        // 16-row kernel: cut[item], one row per sequence; else cut[CTA that began it]
   int whole;          // a CTA to an item: none is cut, no workspace
   unsigned long long limit_ns;
 };

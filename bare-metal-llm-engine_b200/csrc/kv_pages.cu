@@ -1,6 +1,7 @@
 // kv_pages.cu -- the paged 8-bit KV cache: quantising writes, and the pages'
 // bookkeeping (extend, fork, free, compact) on the device, so that a decode loop
 // needs no host round trip and can be captured whole.
+#include <algorithm>
 #include <cmath>
 
 #include "kernels.cuh"
@@ -59,11 +60,11 @@ namespace {
 
 // ---------------------------------------------------------------- write
 //
-// One CTA of 128 threads takes one (page, KV head, K or V): its new rows come
-// in once, 8 halves a thread and pass, and stay in registers between the maximum
-// and the rounding, so a prompt costs 2 bytes read and 1 written per element.
-// The maximum is taken on the bit patterns with the sign cleared: for FP16 these
-// order as the magnitudes do, and anything from 0x7c00 up is an infinity or NaN.
+// A (page, KV head, K | V) tile's new rows come in once, 8 halves a thread and pass, and
+// stay in registers between the maximum and the rounding: 2 bytes read and 1 written
+// per element, which is what bounds a prompt.  The maximum is taken on the bit patterns
+// with the sign cleared: for FP16 these order as the magnitudes do, and anything from
+// 0x7c00 up is an infinity or NaN.
 
 constexpr int kWrThreads = 128;
 
@@ -134,14 +135,64 @@ __device__ int64_t wr_find(const WrParams& p, int64_t item, int* nth) {
   return s_seq;
 }
 
+/// Largest magnitude of 8 halves, as two packed bit patterns.
+__device__ __forceinline__ uint32_t half8_max(const uint4& x) {
+  return __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+}
+
+/// Scale for new rows whose largest magnitude has the bit pattern mx, in a page of scale
+/// `old` (0 for one without earlier rows); NaN where a row is not finite.
+template <bool E4M3>
+__device__ __forceinline__ float wr_scale(uint32_t mx, float old) {
+  constexpr float kQ = E4M3 ? kQMaxE4M3 : kQMaxI8;
+  const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(mx))) * (1.0f / kQ);
+  return mx >= 0x7c00u || old != old ? __int_as_float(0x7fc00000) : fmaxf(s, old);
+}
+
+/// 16 codes times `ratio`, rounded again.
+template <bool E4M3>
+__device__ __forceinline__ uint4 wr_again(const uint4& in, float ratio) {
+  const uint32_t q[4] = {in.x, in.y, in.z, in.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t lo, hi;
+    codes_to_half4<E4M3>(q[j], lo, hi);
+    const float2 f0 = __half22float2(*reinterpret_cast<__half2*>(&lo));
+    const float2 f1 = __half22float2(*reinterpret_cast<__half2*>(&hi));
+    o[j] = to_code<E4M3>(f0.x * ratio) | to_code<E4M3>(f0.y * ratio) << 8 | to_code<E4M3>(f1.x * ratio) << 16 |
+           to_code<E4M3>(f1.y * ratio) << 24;
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+/// 8 halves as codes.  inv = 0 (a NaN scale, or all zeros) gives zeros.
+template <bool E4M3>
+__device__ __forceinline__ uint2 wr_codes(const uint4& x, float inv) {
+  const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+  uint32_t o[2] = {0, 0};
+  if (inv != 0.0f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&in[j]));
+      o[j >> 1] |= (to_code<E4M3>(f.x * inv) | to_code<E4M3>(f.y * inv) << 8) << (16 * (j & 1));
+    }
+  }
+  return make_uint2(o[0], o[1]);
+}
+
+// Several rows: a CTA takes kWrTiles (KV head, K | V) tiles of one page, one after the
+// other with the next one's rows on their way, so that finding the page (three dependent
+// lookups) is paid once for them.
+constexpr int kWrTiles = 4;
+
 template <int PASSES, bool E4M3>
 __global__ void __launch_bounds__(kWrThreads) kv_write_kernel(const WrParams p) {
   pdl_trigger();
   pdl_wait();
-  __shared__ uint32_t s_max[kWrThreads / 32];
+  __shared__ uint32_t s_max[2][kWrThreads / 32];
   int nth = 0;
-  int64_t b = blockIdx.x;
-  if (p.cu != nullptr) b = wr_find(p, blockIdx.x, &nth);
+  const int64_t b = wr_find(p, blockIdx.x, &nth);
   if (b < 0) return;
   int slot, len;
   int64_t r0;
@@ -152,83 +203,104 @@ __global__ void __launch_bounds__(kWrThreads) kv_write_kernel(const WrParams p) 
   const int entry = (start >> p.c.shift) + nth;
   const int page = kv_page(p.c, slot, entry);
   if (page < 0) return;
-  const int first = max(start - entry * page_size, 0);           // first new row in the page
+  const int first = max(start - entry * page_size, 0);  // first new row in the page
   const int rows = min(len - entry * page_size, page_size) - first;
-  const int h = blockIdx.y;
-  const bool is_v = blockIdx.z != 0;
   const int lpr = p.d >> 3;  // threads per row
   const int rpp = kWrThreads / lpr;
   const int tr = threadIdx.x / lpr, tc = (threadIdx.x % lpr) * 8;
-  const __half* src = (is_v ? p.v_new : p.k_new) +
-                      (r0 + (static_cast<int64_t>(entry) * page_size + first - start)) * p.row_pitch +
-                      static_cast<int64_t>(h) * p.d + tc;
-  uint4 x[PASSES];
-  uint32_t mx = 0;
+  const int64_t src0 =
+      (r0 + (static_cast<int64_t>(entry) * page_size + first - start)) * p.row_pitch + tc;
+  const int end = min((static_cast<int>(blockIdx.y) + 1) * kWrTiles, 2 * p.c.heads);
+  auto load = [&](int tile, uint4 (&x)[PASSES]) {
+    const __half* src = ((tile & 1) ? p.v_new : p.k_new) + src0 + static_cast<int64_t>(tile >> 1) * p.d;
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int r = i * rpp + tr;
-    x[i] = r < rows ? __ldg(reinterpret_cast<const uint4*>(src + r * p.row_pitch))
-                    : make_uint4(0, 0, 0, 0);
-    // packed 16-bit maxima of the magnitudes' bit patterns
-    mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu),
-                               __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu)));
+    for (int i = 0; i < PASSES; ++i) {
+      const int r = i * rpp + tr;
+      x[i] = r < rows ? __ldg(reinterpret_cast<const uint4*>(src + r * p.row_pitch)) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  uint4 next[PASSES];
+  int tile = blockIdx.y * kWrTiles;
+  load(tile, next);
+  for (; tile < end; ++tile) {
+    const int h = tile >> 1;
+    const bool is_v = tile & 1;
+    uint4 x[PASSES];
+    uint32_t mx = 0;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      x[i] = next[i];
+      mx = __vmaxu2(mx, half8_max(x[i]));
+    }
+    if (tile + 1 < end) load(tile + 1, next);
+    float* sp = (is_v ? p.c.vs : p.c.ks) + kv_scale_at(p.c, page, h);
+    const float old = first > 0 ? *sp : 0.0f;
+    mx = max(mx & 0xffffu, mx >> 16);
+    mx = __reduce_max_sync(0xffffffffu, mx);
+    if (lane_id() == 0) s_max[tile & 1][threadIdx.x >> 5] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWrThreads / 32; ++w) mx = max(mx, s_max[tile & 1][w]);
+    const float s = wr_scale<E4M3>(mx, old);
+    const float inv = s > 0.0f ? 1.0f / s : 0.0f;  // 0 for NaN: its codes are 0
+    uint8_t* dst = (is_v ? p.c.v : p.c.k) + ((static_cast<int64_t>(page) * p.c.heads + h) << p.c.shift) * p.d;
+    if (first > 0 && s > old) {
+      // The page's other rows, to the larger scale.
+      const float ratio = old / s;
+      uint4* w = reinterpret_cast<uint4*>(dst);
+      const int lo = first * p.d / 16, hi = (first + rows) * p.d / 16;
+      for (int i = threadIdx.x; i < page_size * p.d / 16; i += kWrThreads) {
+        if (i < lo || i >= hi) w[i] = wr_again<E4M3>(w[i], ratio);
+      }
+    }
+    dst += first * p.d + tc;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int r = i * rpp + tr;
+      if (r < rows) *reinterpret_cast<uint2*>(dst + r * p.d) = wr_codes<E4M3>(x[i], inv);
+    }
+    if (threadIdx.x == 0 && (first == 0 || s != old)) *sp = s;
   }
-  mx = max(mx & 0xffffu, mx >> 16);
-  mx = __reduce_max_sync(0xffffffffu, mx);
-  if (lane_id() == 0) s_max[threadIdx.x >> 5] = mx;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWrThreads / 32; ++w) mx = max(mx, s_max[w]);
+}
 
-  constexpr float kQ = E4M3 ? kQMaxE4M3 : kQMaxI8;
+// One row each: d / 8 threads to a (KV head, K | V) row.
+template <bool E4M3>
+__global__ void __launch_bounds__(kWrThreads) kv_append_kernel(const WrParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int lpr = p.d >> 3;
+  const int tile = static_cast<int>(blockIdx.y) * (kWrThreads / lpr) + threadIdx.x / lpr;
+  const int tc = threadIdx.x % lpr;
+  int slot, len;
+  int64_t r0;
+  if (wr_rows(p, blockIdx.x, &slot, &r0, &len) == 0) return;
+  const int page = kv_page(p.c, slot, (len - 1) >> p.c.shift);
+  if (page < 0) return;
+  const int first = (len - 1) & ((1 << p.c.shift) - 1);
+  const bool live = tile < 2 * p.c.heads, is_v = tile & 1;
+  const int h = live ? tile >> 1 : 0;
+  const __half* src = (is_v ? p.v_new : p.k_new) + r0 * p.row_pitch + static_cast<int64_t>(h) * p.d + tc * 8;
+  const uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
   float* sp = (is_v ? p.c.vs : p.c.ks) + kv_scale_at(p.c, page, h);
-  const float old = first > 0 ? *sp : 0.0f;
-  float s = __half2float(__ushort_as_half(static_cast<unsigned short>(mx))) * (1.0f / kQ);
-  if (mx >= 0x7c00u || old != old) s = __int_as_float(0x7fc00000);
-  else s = fmaxf(s, old);
-  const float inv = s > 0.0f ? 1.0f / s : 0.0f;  // 0 for NaN: its codes are 0
-  uint8_t* tile = (is_v ? p.c.v : p.c.k) +
-                  ((static_cast<int64_t>(page) * p.c.heads + h) << p.c.shift) * p.d;
+  const float old = live && first > 0 ? *sp : 0.0f;
+  uint32_t mx = half8_max(x);
+  mx = max(mx & 0xffffu, mx >> 16);
+  for (int o = 1; o < lpr; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  __syncwarp();
+  if (!live) return;
+  const float s = wr_scale<E4M3>(mx, old);
+  const float inv = s > 0.0f ? 1.0f / s : 0.0f;
+  uint8_t* dst = (is_v ? p.c.v : p.c.k) + ((static_cast<int64_t>(page) * p.c.heads + h) << p.c.shift) * p.d;
   if (first > 0 && s > old) {
-    // The page's other rows, to the larger scale.
     const float ratio = old / s;
-    uint4* w = reinterpret_cast<uint4*>(tile);
-    const int lo = first * p.d / 16, hi = (first + rows) * p.d / 16;
-    for (int i = threadIdx.x; i < page_size * p.d / 16; i += kWrThreads) {
-      if (i >= lo && i < hi) continue;
-      const uint4 in = w[i];
-      const uint32_t q[4] = {in.x, in.y, in.z, in.w};
-      uint32_t o[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t lo, hi;
-        codes_to_half4<E4M3>(q[j], lo, hi);
-        const float2 f0 = __half22float2(*reinterpret_cast<__half2*>(&lo));
-        const float2 f1 = __half22float2(*reinterpret_cast<__half2*>(&hi));
-        o[j] = to_code<E4M3>(f0.x * ratio) | to_code<E4M3>(f0.y * ratio) << 8 |
-               to_code<E4M3>(f1.x * ratio) << 16 | to_code<E4M3>(f1.y * ratio) << 24;
-      }
-      w[i] = make_uint4(o[0], o[1], o[2], o[3]);
+    uint4* w = reinterpret_cast<uint4*>(dst);
+    const int lo = first * p.d / 16, hi = (first + 1) * p.d / 16;
+    for (int i = tc; i < (p.d << p.c.shift) / 16; i += lpr) {
+      if (i < lo || i >= hi) w[i] = wr_again<E4M3>(w[i], ratio);
     }
   }
-  uint8_t* dst = tile + first * p.d + tc;
-#pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int r = i * rpp + tr;
-    if (r < rows) {
-      const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      uint32_t o[2] = {0, 0};
-      if (s == s) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&in[j]));
-          o[j >> 1] |= (to_code<E4M3>(f.x * inv) | to_code<E4M3>(f.y * inv) << 8) << (16 * (j & 1));
-        }
-      }
-      *reinterpret_cast<uint2*>(dst + r * p.d) = make_uint2(o[0], o[1]);
-    }
-  }
-  if (threadIdx.x == 0 && (first == 0 || s != old)) *sp = s;
+  *reinterpret_cast<uint2*>(dst + first * p.d + tc * 8) = wr_codes<E4M3>(x, inv);
+  if (tc == 0 && (first == 0 || s != old)) *sp = s;
 }
 
 template <int PASSES>
@@ -527,9 +599,11 @@ __global__ void __launch_bounds__(kBkThreads) kv_compact_kernel(const BkParams p
 
 // ---------------------------------------------------------------- page copies
 //
-// A page's codes are contiguous in each layer (all heads), so a copy is blocks of
-// page_size * n_kv_heads * head_dim bytes; 16 bytes a thread, grid-stride over
-// (pair, layer, K | V, 16-byte word).
+// A page's codes are contiguous in each layer (all heads): a copy is a block of page_size *
+// n_kv_heads * head_dim bytes for each pair, layer and K | V.  CTAs stride over chunks of
+// 16 KB, every thread with four 16-byte loads on their way before it stores.
+constexpr int kCpThreads = 256, kCpUnroll = 4;
+constexpr int kCpChunk = kCpThreads * kCpUnroll;  // 16-byte words
 
 struct CpParams {
   uint8_t* k;
@@ -547,35 +621,40 @@ struct CpParams {
   int64_t entries;
 };
 
-__global__ void __launch_bounds__(256) kv_copy_kernel(const CpParams p) {
+__global__ void __launch_bounds__(kCpThreads) kv_copy_kernel(const CpParams p) {
   pdl_trigger();
   pdl_wait();
-  const int64_t t0 = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
-  const int64_t nt = static_cast<int64_t>(gridDim.x) * blockDim.x;
   if (p.table != nullptr) {
-    for (int64_t i = t0; i < p.entries; i += nt) {
+    const int64_t nt = static_cast<int64_t>(gridDim.x) * kCpThreads;
+    for (int64_t i = blockIdx.x * static_cast<int64_t>(kCpThreads) + threadIdx.x; i < p.entries; i += nt) {
       const int id = p.table[i];
       if (id >= 0 && id < p.n_pages) p.table[i] = p.remap[id];
     }
   }
-  const int64_t n = *p.n_pairs;
-  const int64_t total = n * p.layers * 2 * p.words;
-  for (int64_t i = t0; i < total; i += nt) {
-    const int64_t block = i / p.words, w = i - block * p.words;
+  const int64_t chunks = (p.words + kCpChunk - 1) / kCpChunk;  // of a block
+  const int64_t total = static_cast<int64_t>(*p.n_pairs) * p.layers * 2 * chunks;
+  for (int64_t u = blockIdx.x; u < total; u += gridDim.x) {
+    const int64_t block = u / chunks, part = u - block * chunks;
     const int64_t pl = block >> 1;
     const int64_t pair = pl / p.layers, layer = pl - pair * p.layers;
     const int2 m = p.pairs[pair];
-    uint4* base = reinterpret_cast<uint4*>((block & 1) ? p.v : p.k);
-    base[(layer * p.n_pages + m.y) * p.words + w] = base[(layer * p.n_pages + m.x) * p.words + w];
-  }
-  const int64_t scales = n * p.layers * 2 * p.heads;
-  for (int64_t i = t0; i < scales; i += nt) {
-    const int64_t block = i / p.heads, h = i - block * p.heads;
-    const int64_t pl = block >> 1;
-    const int64_t pair = pl / p.layers, layer = pl - pair * p.layers;
-    const int2 m = p.pairs[pair];
-    float* base = (block & 1) ? p.vs : p.ks;
-    base[(layer * p.n_pages + m.y) * p.heads + h] = base[(layer * p.n_pages + m.x) * p.heads + h];
+    const uint4* src = reinterpret_cast<const uint4*>((block & 1) ? p.v : p.k) + (layer * p.n_pages + m.x) * p.words;
+    uint4* dst = reinterpret_cast<uint4*>((block & 1) ? p.v : p.k) + (layer * p.n_pages + m.y) * p.words;
+    const int64_t w0 = part * kCpChunk + threadIdx.x;
+    uint4 x[kCpUnroll];
+#pragma unroll
+    for (int i = 0; i < kCpUnroll; ++i) {
+      if (w0 + i * kCpThreads < p.words) x[i] = __ldcs(src + w0 + i * kCpThreads);
+    }
+    if (part == 0) {
+      float* base = (block & 1) ? p.vs : p.ks;
+      for (int h = threadIdx.x; h < p.heads; h += kCpThreads)
+        base[(layer * p.n_pages + m.y) * p.heads + h] = base[(layer * p.n_pages + m.x) * p.heads + h];
+    }
+#pragma unroll
+    for (int i = 0; i < kCpUnroll; ++i) {
+      if (w0 + i * kCpThreads < p.words) __stcs(dst + w0 + i * kCpThreads, x[i]);
+    }
   }
 }
 
@@ -611,12 +690,10 @@ int launch_copy(const engine_kv_pages_t* kv, const int2* pairs, const int32_t* n
   c.table = table;
   c.remap = remap;
   c.entries = table != nullptr ? kv->n_slots * kv->max_pages : 0;
-  int64_t units = most * kv->n_layers * 2 * c.words;
-  if (units < c.entries) units = c.entries;
-  const int64_t cap = static_cast<int64_t>(sm_count()) * 8;
-  const int64_t blocks = (units + 255) / 256;
-  B200_CUDA(launch_pdl(kv_copy_kernel, dim3(static_cast<unsigned>(blocks < cap ? blocks : cap)),
-                       dim3(256), 0, st, c));
+  int64_t blocks = most * kv->n_layers * 2 * ((c.words + kCpChunk - 1) / kCpChunk);
+  blocks = std::max(blocks, (c.entries + kCpThreads - 1) / kCpThreads);
+  blocks = std::min(blocks, static_cast<int64_t>(sm_count()) * 8);
+  B200_CUDA(launch_pdl(kv_copy_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kCpThreads), 0, st, c));
   return ENGINE_OK;
 }
 
@@ -665,16 +742,24 @@ int engine_cuda_kv_pages_write(const engine_kv_pages_t* kv, int64_t layer,
   p.n_seq = n_seq;
   p.n_tokens = n_tokens;
   p.d = static_cast<int>(kv->head_dim);
-  const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>(kv->n_kv_heads), 2);
   const bool e4m3 = kv->type == ENGINE_KV_E4M3;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // 1024 elements a pass; one row is one pass.
-  const int64_t passes = cu_new == nullptr ? 1 : kv->page_size * kv->head_dim / 1024;
-  const int rc = passes <= 1   ? launch_write<1>(p, grid, e4m3, st)
-                 : passes <= 2 ? launch_write<2>(p, grid, e4m3, st)
-                 : passes <= 4 ? launch_write<4>(p, grid, e4m3, st)
-                 : passes <= 8 ? launch_write<8>(p, grid, e4m3, st)
-                               : launch_write<16>(p, grid, e4m3, st);
+  int rc = ENGINE_OK;
+  const int64_t tiles = 2 * kv->n_kv_heads;
+  if (cu_new == nullptr) {
+    const int64_t per = kWrThreads / (kv->head_dim / 8);
+    const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>((tiles + per - 1) / per));
+    B200_CUDA(e4m3 ? launch_pdl(kv_append_kernel<true>, grid, dim3(kWrThreads), 0, st, p)
+                   : launch_pdl(kv_append_kernel<false>, grid, dim3(kWrThreads), 0, st, p));
+  } else {
+    const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>((tiles + kWrTiles - 1) / kWrTiles));
+    const int64_t passes = kv->page_size * kv->head_dim / 1024;  // 1024 elements each
+    rc = passes <= 1   ? launch_write<1>(p, grid, e4m3, st)
+         : passes <= 2 ? launch_write<2>(p, grid, e4m3, st)
+         : passes <= 4 ? launch_write<4>(p, grid, e4m3, st)
+         : passes <= 8 ? launch_write<8>(p, grid, e4m3, st)
+                       : launch_write<16>(p, grid, e4m3, st);
+  }
   if (rc != ENGINE_OK) return rc;
   return check_launch("kv_pages_write");
   B200_ENTRY_END

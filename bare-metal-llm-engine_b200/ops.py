@@ -296,6 +296,7 @@ class PagedKV:
         self.table, self.length, self.ref = table, length, ref
         self.n_slots, self.max_pages = table.shape
         self.n_kv_heads, self.head_dim, self.n_pages = hk, d, n_pages
+        self.width = hk * d
         self.device_index = k.device.index
         self.desc = _KvPages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                              table.data_ptr(), length.data_ptr(), ref.data_ptr(), n_layers, n_pages,
@@ -316,21 +317,31 @@ class PagedKV:
                    torch.zeros(n_pages, **z))
 
 
-def _kv_req(kv, *named):
-    """The calls' checks: the cache on the current device, int32 arguments beside it."""
-    if kv.device_index != torch.cuda.current_device():
+def _kv_stream(kv) -> int:
+    """The current stream of the cache's device, which has to be the current device.  (The raw
+    handle: torch.cuda.current_stream() builds an object, 3 us, as long as a small call.)"""
+    if kv.device_index != torch._C._cuda_getDevice():
         raise ValueError(f"the cache is on cuda:{kv.device_index}, which is not the current device")
-    for t, n in named:
-        _req(t, torch.int32, n)
-        if t.device.index != kv.device_index:
-            raise ValueError(f"{n} must be on the cache's device")
+    return torch._C._cuda_getCurrentRawStream(kv.device_index)
 
 
-def _kv_slots(kv, slots, n):
-    """Entries of a call over `slots` (None: slots 0 .. n - 1)."""
-    if slots is not None and slots.numel() != n:
+def _kv_i32(kv, t, name: str) -> int:
+    """Address of an int32 tensor on the cache's device."""
+    if type(t) is not torch.Tensor or t.dtype is not torch.int32 or t.get_device() != kv.device_index \
+            or not t.is_contiguous():
+        _req(t, torch.int32, name)
+        if t.get_device() != kv.device_index:
+            raise ValueError(f"{name} must be on the cache's device")
+    return t.data_ptr()
+
+
+def _kv_slots(kv, slots, n) -> int:
+    """Address of the slots of a call over n entries (None: slots 0 .. n - 1)."""
+    if slots is None:
+        return 0
+    if slots.numel() != n:
         raise ValueError(f"slots must have {n} entries, got {slots.numel()}")
-    return _ptr(slots)
+    return _kv_i32(kv, slots, "slots")
 
 
 def kv_pages_extend(kv, slots, n_new):
@@ -338,39 +349,47 @@ def kv_pages_extend(kv, slots, n_new):
     taking the pages they need, lowest free id first.  Returns status [1] int32:
     0, or the number of missing pages, or -1 for a bad argument; unless 0, nothing
     changed.  Nothing is synchronised: read the status when it is wanted."""
-    _kv_req(kv, (n_new, "n_new"), *(() if slots is None else ((slots, "slots"),)))
-    status = torch.empty(1, device=n_new.device, dtype=torch.int32)
+    st = _kv_stream(kv)
     n = n_new.numel()
-    _c.kv_pages_extend(kv.handle, _kv_slots(kv, slots, n), n_new.data_ptr(), status.data_ptr(), n,
-                       _stream())
+    add = _kv_i32(kv, n_new, "n_new")
+    status = torch.empty(1, device=n_new.device, dtype=torch.int32)
+    _c.kv_pages_extend(kv.handle, _kv_slots(kv, slots, n), add, status.data_ptr(), n, st)
     return status
 
 
 def kv_pages_fork(kv, parents, children):
     """Makes the empty slots children[i] copies of parents[i]: full pages shared, the
     partly filled one copied in all layers.  Returns status as kv_pages_extend."""
-    _kv_req(kv, (parents, "parents"), (children, "children"))
-    if parents.numel() != children.numel():
+    st = _kv_stream(kv)
+    par, chi = _kv_i32(kv, parents, "parents"), _kv_i32(kv, children, "children")
+    n = parents.numel()
+    if n != children.numel():
         raise ValueError("parents and children must have as many entries")
     status = torch.empty(1, device=parents.device, dtype=torch.int32)
-    _c.kv_pages_fork(kv.handle, parents.data_ptr(), children.data_ptr(), status.data_ptr(),
-                     parents.numel(), _stream())
+    _c.kv_pages_fork(kv.handle, par, chi, status.data_ptr(), n, st)
     return status
 
 
 def kv_pages_free(kv, slots):
     """Empties the slots; pages without a user left are free again."""
-    _kv_req(kv, (slots, "slots"))
-    _c.kv_pages_free(kv.handle, slots.data_ptr(), slots.numel(), _stream())
+    st = _kv_stream(kv)
+    _c.kv_pages_free(kv.handle, _kv_i32(kv, slots, "slots"), slots.numel(), st)
 
 
 def kv_pages_compact(kv):
     """Moves the pages in use to the lowest ids, in all layers; tables and ref follow.
     Returns remap [n_pages] int32: the new id of each page, -1 if it was free."""
-    _kv_req(kv)
+    st = _kv_stream(kv)
     remap = torch.empty(kv.n_pages, device=kv.ref.device, dtype=torch.int32)
-    _c.kv_pages_compact(kv.handle, remap.data_ptr(), _stream())
+    _c.kv_pages_compact(kv.handle, remap.data_ptr(), st)
     return remap
+
+
+def _kv_f16(kv, t, name):
+    if t.dtype is not torch.float16 or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA float16 tensor")
+    if t.get_device() != kv.device_index:
+        raise ValueError(f"{name} must be on the cache's device")
 
 
 def kv_pages_write(kv, layer: int, k_rows, v_rows, slots=None, cu_new=None):
@@ -378,55 +397,51 @@ def kv_pages_write(kv, layer: int, k_rows, v_rows, slots=None, cu_new=None):
     columns of a fused Q/K/V projection) as the LAST positions of the slots: rows
     [cu_new[i], cu_new[i+1]) of slot slots[i], or one row each where cu_new is None.
     Call kv_pages_extend first: it counts them."""
-    _kv_req(kv, *(() if slots is None else ((slots, "slots"),)),
-            *(() if cu_new is None else ((cu_new, "cu_new"),)))
-    for t, n in ((k_rows, "k_rows"), (v_rows, "v_rows")):
-        if t.dtype != torch.float16 or not t.is_cuda:
-            raise TypeError(f"{n} must be a CUDA float16 tensor")
-        if t.dim() != 2 or t.shape[1] != kv.n_kv_heads * kv.head_dim:
-            raise ValueError(f"{n} must be [n_tokens, H_kv * d]")
-        if t.device.index != kv.device_index:
-            raise ValueError(f"{n} must be on the cache's device")
-    if k_rows.shape != v_rows.shape or k_rows.stride() != v_rows.stride() or k_rows.stride(1) != 1:
+    st = _kv_stream(kv)
+    _kv_f16(kv, k_rows, "k_rows")
+    _kv_f16(kv, v_rows, "v_rows")
+    shape, stride = k_rows.shape, k_rows.stride()
+    if len(shape) != 2 or shape[1] != kv.width:
+        raise ValueError("k_rows must be [n_tokens, H_kv * d]")
+    if v_rows.shape != shape or v_rows.stride() != stride or stride[1] != 1:
         raise ValueError("k_rows / v_rows: rows must be contiguous, as many, and share one pitch")
-    n_tokens = k_rows.shape[0]
-    n_seq = n_tokens if cu_new is None else cu_new.numel() - 1
-    pitch = k_rows.stride(0) if n_tokens > 1 else max(k_rows.stride(0), k_rows.shape[1])
-    _c.kv_pages_write(kv.handle, layer, k_rows.data_ptr(), v_rows.data_ptr(), pitch,
-                      _kv_slots(kv, slots, n_seq), _ptr(cu_new), n_seq, n_tokens, _stream())
+    n_tokens = shape[0]
+    n_seq, cu = n_tokens, 0
+    if cu_new is not None:
+        n_seq, cu = cu_new.numel() - 1, _kv_i32(kv, cu_new, "cu_new")
+    _c.kv_pages_write(kv.handle, layer, k_rows.data_ptr(), v_rows.data_ptr(),
+                      stride[0] if n_tokens > 1 else max(stride[0], kv.width),
+                      _kv_slots(kv, slots, n_seq), cu, n_seq, n_tokens, st)
 
 
 def _paged_q(kv, q, out):
-    """Checks q [n, H, d] (heads contiguous, rows may be strided) and out; (pitch, out)."""
-    if q.dtype != torch.float16 or not q.is_cuda:
-        raise TypeError("q must be a CUDA float16 tensor")
-    if q.dim() != 3 or q.shape[2] != kv.head_dim:
+    """Checks q [n, H, d] (heads contiguous, rows may be strided) and out; (n, H, pitch, out)."""
+    _kv_f16(kv, q, "q")
+    shape, stride = q.shape, q.stride()
+    if len(shape) != 3 or shape[2] != kv.head_dim:
         raise ValueError("q must be [n, H, d]")
-    if q.device.index != kv.device_index:
-        raise ValueError("q must be on the cache's device")
-    n, H, d = q.shape
-    if q.stride(2) != 1 or (H > 1 and q.stride(1) != d):
+    n, H, d = shape
+    if stride[2] != 1 or (H > 1 and stride[1] != d):
         raise ValueError("q: the heads of a row must be contiguous")
     if out is None:
-        out = torch.empty(q.shape, device=q.device, dtype=torch.float16)
+        out = torch.empty(shape, device=q.device, dtype=torch.float16)
     else:
         _req(out, torch.float16, "out")
-        if out.shape != q.shape:
-            raise ValueError("out must have q's shape")
-    return (q.stride(0) if n > 1 else max(q.stride(0), H * d)), out
+        if out.shape != shape or out.get_device() != kv.device_index:
+            raise ValueError("out must have q's shape and device")
+    return n, H, (stride[0] if n > 1 else max(stride[0], H * d)), out
 
 
 def attention_paged_decode(kv, layer: int, q, slots=None, scale=None, out=None,
                            want_lse: bool = False):
     """out [B, H, d] of one query row per sequence, q [B, H, d], over all positions of
     the slots (None: slots 0 .. B - 1); with want_lse also lse [B, H] (FP32)."""
-    _kv_req(kv, *(() if slots is None else ((slots, "slots"),)))
-    pitch, o = _paged_q(kv, q, out)
-    B, H, d = q.shape
+    st = _kv_stream(kv)
+    B, H, pitch, o = _paged_q(kv, q, out)
     lse = torch.empty(B, H, device=q.device, dtype=torch.float32) if want_lse else None
     _c.attention_paged_decode(kv.handle, layer, q.data_ptr(), pitch, _kv_slots(kv, slots, B),
-                              o.data_ptr(), _ptr(lse), B, H, d ** -0.5 if scale is None else scale,
-                              _stream())
+                              o.data_ptr(), _ptr(lse), B, H,
+                              kv.head_dim ** -0.5 if scale is None else scale, st)
     return (o, lse) if want_lse else o
 
 
@@ -436,14 +451,13 @@ def attention_paged_prefill(kv, layer: int, q, slots, cu_q, scale=None, out=None
     positions of slot slots[i] (None: slot i), over the slot's positions up to their
     own (all of them unless is_causal).  Rows past cu_q[-1] are left as they were in
     `out`.  With want_lse also lse [T, H] (FP32)."""
-    _kv_req(kv, (cu_q, "cu_q"), *(() if slots is None else ((slots, "slots"),)))
-    pitch, o = _paged_q(kv, q, out)
-    T, H, d = q.shape
-    n_seq = cu_q.numel() - 1
+    st = _kv_stream(kv)
+    T, H, pitch, o = _paged_q(kv, q, out)
+    n_seq, cu = cu_q.numel() - 1, _kv_i32(kv, cu_q, "cu_q")
     lse = torch.empty(T, H, device=q.device, dtype=torch.float32) if want_lse else None
     _c.attention_paged_prefill(kv.handle, layer, q.data_ptr(), pitch, _kv_slots(kv, slots, n_seq),
-                               cu_q.data_ptr(), o.data_ptr(), _ptr(lse), n_seq, T, H,
-                               d ** -0.5 if scale is None else scale, is_causal, _stream())
+                               cu, o.data_ptr(), _ptr(lse), n_seq, T, H,
+                               kv.head_dim ** -0.5 if scale is None else scale, is_causal, st)
     return (o, lse) if want_lse else o
 
 

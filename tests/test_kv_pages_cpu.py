@@ -110,6 +110,34 @@ def test_paged_kv_checks_its_tensors(pkg):
         pkg.ops.PagedKV(**{**good, "k": good["k"][0], "v": good["v"][0]})
 
 
+def test_calls_check_their_tensors(pkg, monkeypatch):
+    """Another current device, other types, shapes and strides: refused in Python, with a
+    stand-in for the cache (nothing reaches the library)."""
+    from types import SimpleNamespace
+
+    ops = pkg.ops
+    kv = SimpleNamespace(device_index=1, handle=0, width=128, head_dim=64, n_pages=4)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 0, raising=False)
+    i = torch.zeros(2, dtype=torch.int32)
+    h = torch.zeros(2, 128).half()
+    for call in (lambda: ops.kv_pages_extend(kv, i, i), lambda: ops.kv_pages_fork(kv, i, i),
+                 lambda: ops.kv_pages_free(kv, i), lambda: ops.kv_pages_compact(kv),
+                 lambda: ops.kv_pages_write(kv, 0, h, h), lambda: ops.attention_paged_decode(kv, 0, h),
+                 lambda: ops.attention_paged_prefill(kv, 0, h, None, i)):
+        with pytest.raises(ValueError, match="not the current device"):
+            call()
+    kv.device_index = 0
+    with pytest.raises(ValueError, match="n_new must be a CUDA tensor"):
+        ops.kv_pages_extend(kv, None, i)
+    with pytest.raises(ValueError, match="slots must be a CUDA tensor"):
+        ops.kv_pages_free(kv, i)
+    with pytest.raises(TypeError, match="k_rows must be a CUDA float16"):
+        ops.kv_pages_write(kv, 0, h, h)
+    with pytest.raises(TypeError, match="q must be a CUDA float16"):
+        ops.attention_paged_decode(kv, 0, h)
+
+
 @pytest.mark.parametrize("dtype", [torch.int8, torch.float8_e4m3fn])
 def test_restatement_rounds_to_the_nearest(dtype):
     """The Model's codes: each value within half a step of what was written, also after
