@@ -45,6 +45,10 @@ constexpr int kPgConsumers = 4;  // warps; each takes 16 keys of a tile
 constexpr int kPgThreads = (kPgConsumers + 1) * 32;
 constexpr int kPgMaxSeq = 1024;  // sequences per launch (their prefix sums sit in shared memory)
 constexpr float kPgRescale = 8.0f;
+/// What an item costs beside its key tiles (its q, the chain of its first tile, the join of
+/// the warps), in tiles: the even shares count it, as steps in front of the item's tiles in
+/// which nothing is done.
+constexpr int kPgItemCost = 3;
 constexpr int64_t kManyRows = 32;  // from here on attention_paged_tc
 constexpr int64_t kWholeTiles = 16;  // slots of at most so many tiles: a CTA to an item
 static_assert(kPgMaxSeq <= kTcMaxSeq, "both kernels take a launch's sequences");
@@ -56,10 +60,11 @@ struct PgCfg {
   static constexpr int kRows = 8 * NQ;
   static constexpr int kCtas = 3;
   static constexpr int kTile = kPgKeys * D;  // bytes of K (or V) of a tile
-  static constexpr int kStages = (NQ == 1 ? 4 : 3) * 128 / D * (D == 128 ? 4 : 3) / 4;
+  static constexpr int kStages = D == 128 ? 3 : 5;
   static constexpr int kOW = D + 4;          // pitch of a row of O in shared memory
+  static constexpr int kBufs = 4 / NQ;       // copies of it: warps to a copy one after the other
   static constexpr int kOffO = kStages * 2 * kTile;
-  static constexpr int kOffQ = kOffO + kRows * kOW * 4;       // [D / 16][32 lanes], 16 bytes each
+  static constexpr int kOffQ = kOffO + kBufs * kRows * kOW * 4;  // [D / 16][32 lanes], 16 bytes each
   static constexpr int kOffConst = kOffQ + (NQ == 1 ? 0 : D / 16 * 512);
   static constexpr int kOffBar = kOffConst + kStages * 4 * 16;
   static constexpr int kOffMl = kOffBar + 2 * kStages * 8;
@@ -129,18 +134,19 @@ struct PgItem {
   int n_rows;    // flat rows of the sequence
   int n_tok;     // its tokens
   int64_t first; // its first token
-  int t0, t1;    // tiles
-  int begin;     // the item's first tile, counted over all items
+  int t0, t1;    // tiles; none where the share ends within the item's leading steps
+  int begin;     // the item's first step, counted over all items
+  int end;       // the step behind this part
   int tiles;     // of the whole item
 };
 
 struct PgLists {
-  const int32_t* pre;   // tiles before each sequence
+  const int32_t* pre;   // steps before each sequence
   const int32_t* slot;
   const int32_t* len;
 };
 
-/// The item at tile `x` (`whole`: the item of that number), up to tile `hi`.
+/// The item at step `x` (`whole`: the item of that number), up to step `hi`.
 __device__ __forceinline__ PgItem pg_item(const ApParams& p, const PgLists& s, int x, int hi) {
   int lo = 0, up = p.n_seq - 1;
   while (lo < up) {  // the last sequence that starts at or before x
@@ -154,10 +160,12 @@ __device__ __forceinline__ PgItem pg_item(const ApParams& p, const PgLists& s, i
   it.len = s.len[lo];
   it.tiles = max((it.len + kPgKeys - 1) / kPgKeys, 1);
   const int y = x - s.pre[lo];
-  const int j = p.whole ? y : y / it.tiles;
-  it.t0 = p.whole ? 0 : y - j * it.tiles;
-  it.t1 = p.whole ? it.tiles : min(it.tiles, it.t0 + hi - x);
-  it.begin = x - it.t0;
+  const int steps = p.whole ? 1 : kPgItemCost + it.tiles;
+  const int j = y / steps;
+  it.begin = s.pre[lo] + j * steps;
+  it.t0 = p.whole ? 0 : max(x - it.begin - kPgItemCost, 0);
+  it.t1 = p.whole ? it.tiles : max(min(hi - it.begin - kPgItemCost, it.tiles), it.t0);
+  it.end = it.begin + (p.whole ? 1 : kPgItemCost + it.t1);
   it.head = j % p.c.heads;
   it.row0 = j / p.c.heads * kPgRows;
   it.n_tok = kv_rows(p.c, p.cu, p.seq0 + lo, p.n_tokens, &it.first);
@@ -202,7 +210,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
   }
   pdl_trigger();
   pdl_wait();
-  // Tiles of each sequence, then their sums.
+  // Steps of each sequence, then their sums.
   for (int b = threadIdx.x; b < p.n_seq; b += kPgThreads) {
     const int slot = kv_slot(p.c, p.slots, p.seq0 + b);
     const int len = kv_length(p.c, slot);
@@ -210,7 +218,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
     const int rows = kv_rows(p.c, p.cu, p.seq0 + b, p.n_tokens, &first) * p.group;
     s_slot[b] = slot;
     s_len[b] = len;
-    s_pre[b] = (rows + kPgRows - 1) / kPgRows * p.c.heads * (p.whole ? 1 : max((len + kPgKeys - 1) / kPgKeys, 1));
+    s_pre[b] = (rows + kPgRows - 1) / kPgRows * p.c.heads * (p.whole ? 1 : kPgItemCost + max((len + kPgKeys - 1) / kPgKeys, 1));
   }
   __syncthreads();
   if (warp == 0) {
@@ -231,7 +239,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
   __syncthreads();
   const PgLists lists{s_pre, s_slot, s_len};
   const int total = s_pre[p.n_seq];
-  // Tiles (items, where `whole`) to a CTA.
+  // Steps (items, where `whole`) to a CTA.
   const int per = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
   const int lo = min(static_cast<int64_t>(blockIdx.x) * per, static_cast<int64_t>(total));
   const int hi = min(lo + per, total);
@@ -244,14 +252,24 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
     bool ok = true;
     for (int x = lo; x < hi && ok;) {
       const PgItem it = pg_item(p, lists, x, hi);
-      x += p.whole ? 1 : it.t1 - it.t0;
+      x = it.end;
+      if (it.t0 == it.t1) break;
       const int n_keys = it.len;
       const int first_slice = it.t0 * 4, end_slice = min(it.t1 * 4, (n_keys + 15) >> 4);
-      // Lane i of batch k looks after slice first_slice + 32 k + i.
-      auto page_of = [&](int slice) {
-        return slice < end_slice ? kv_page(p.c, it.slot, (slice << 4) >> p.c.shift) : -1;
+      // Lane i of batch k looks after slice first_slice + 32 k + i.  Entries and scales are read
+      // a batch ahead, and checked only when they are wanted.
+      auto entry_of = [&](int slice) {
+        return slice < end_slice
+                   ? p.c.table[static_cast<int64_t>(it.slot) * p.c.max_pages + ((slice << 4) >> p.c.shift)]
+                   : -1;
       };
-      int id = page_of(first_slice + lane), id1 = page_of(first_slice + 32 + lane);
+      auto checked = [&](int id, int slice) {
+        if (id >= 0 && id < p.c.n_pages) return id;
+        if (slice < end_slice) atomicOr(p.c.err, kErrBadArgument);
+        return -1;
+      };
+      int id = entry_of(first_slice + lane), id1 = entry_of(first_slice + 32 + lane);
+      id = checked(id, first_slice + lane);
       float ks = 0.0f, vs = 0.0f, ks1 = 0.0f, vs1 = 0.0f;
       if (id >= 0) {
         ks = p.c.ks[kv_scale_at(p.c, id, it.head)];
@@ -286,14 +304,10 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
         if (n == 0) {
           for (; ahead < min(count, ST) && ok; ++ahead) fetch(ahead, ahead);
         }
-        const int id2 = page_of((base + 16) * 4 + lane);
-        if (id1 >= 0) {
-          ks1 = p.c.ks[kv_scale_at(p.c, id1, it.head)];
-          vs1 = p.c.vs[kv_scale_at(p.c, id1, it.head)];
-        }
         const float v1 = vs == 0.0f ? 1.0f : vs;
         const float4 con = id >= 0 ? make_float4(ks * kc_unit, log2f(v1), 1.0f / v1, 1.0f)
                                    : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+        int id2 = -1;
         for (int i = 0; i < count && ok; ++i, ++n) {
           if (i >= ahead) fetch(n, i);
           if (!ok) break;
@@ -301,6 +315,14 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
           if (lane >> 2 == i) s_const[s * 4 + (lane & 3)] = con;
           __syncwarp();
           if (lane == 0) mbar_arrive(&full[s]);
+          if (i == min(ahead, count - 1)) {  // the next batch's scales, and the entries behind it
+            id2 = entry_of((base + 16) * 4 + lane);
+            id1 = checked(id1, (base + 8) * 4 + lane);
+            if (id1 >= 0) {
+              ks1 = p.c.ks[kv_scale_at(p.c, id1, it.head)];
+              vs1 = p.c.vs[kv_scale_at(p.c, id1, it.head)];
+            }
+          }
         }
         issued = max(n, ahead);
         id = id1;
@@ -327,7 +349,8 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
     if (threadIdx.x == 0 && !p.whole && !p.by_item) p.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
     for (int x = lo; x < hi;) {
       const PgItem it = pg_item(p, lists, x, hi);
-      x += p.whole ? 1 : it.t1 - it.t0;
+      x = it.end;
+      if (it.t0 == it.t1) break;
       // q^T as B fragments: the lane's D / 4 elements of query row g (and g + 8), from
       // t * D / 4.  In the sums' columns a lane has rows 2t and 2t + 1 (and + 8).
       uint32_t bq[NQ == 1 ? NK : 1][2];
@@ -555,13 +578,14 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
           a[nq][e] = m[nq][e] == -INFINITY ? (l[nq][e] != l[nq][e] ? l[nq][e] : 0.0f) : ex2_approx(m[nq][e] - mm);
         }
       }
-      for (int w = 0; w < kPgConsumers; ++w) {
-        if (warp == w) {
+#pragma unroll
+      for (int w = 0; w < kPgConsumers / Cfg::kBufs; ++w) {
+        if (warp / Cfg::kBufs == w) {
 #pragma unroll
           for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float* row = s_o + (8 * nq + 2 * t + e) * Cfg::kOW + g * (D / 8);
+              float* row = s_o + ((warp % Cfg::kBufs) * Cfg::kRows + 8 * nq + 2 * t + e) * Cfg::kOW + g * (D / 8);
 #pragma unroll
               for (int j = 0; j < NK; j += 2) {
                 float4* dst = reinterpret_cast<float4*>(row + 2 * j);
@@ -592,7 +616,12 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
           if (e.x != -INFINITY) ll = fmaf(e.y, ex2_approx(e.x - mm), ll);
           else if (e.y != e.y) ll = e.y;  // a NaN weight
         }
-        const float4 u = *reinterpret_cast<const float4*>(s_o + row * Cfg::kOW + col);
+        float4 u = *reinterpret_cast<const float4*>(s_o + row * Cfg::kOW + col);
+#pragma unroll
+        for (int w = 1; w < Cfg::kBufs; ++w) {
+          const float4 y = *reinterpret_cast<const float4*>(s_o + (w * Cfg::kRows + row) * Cfg::kOW + col);
+          u = make_float4(u.x + y.x, u.y + y.y, u.z + y.z, u.w + y.w);
+        }
         if (whole) {
           if (!ok) continue;
           const int64_t at = pg_row(p, it.first, it.head, it.row0 + row);
@@ -607,7 +636,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
         }
       }
       if (threadIdx.x == 0 && it.t0 == 0 && !p.whole && (p.by_item || !whole)) {
-        const int parts = (it.begin + it.tiles - 1) / per - static_cast<int>(blockIdx.x) + 1;
+        const int parts = (it.begin + kPgItemCost + it.tiles - 1) / per - static_cast<int>(blockIdx.x) + 1;
         const int at = p.by_item ? (it.b * ((p.group + kPgRows - 1) / kPgRows) + it.row0 / kPgRows) * p.c.heads + it.head
                                  : static_cast<int>(blockIdx.x);
         p.cut[at] = make_int4(whole ? -1 : it.b, it.row0, it.head | parts << 16, static_cast<int>(blockIdx.x));
@@ -621,19 +650,23 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
 /// up to that which finished it); blockIdx.x is the entry of p.cut, blockIdx.y the row.  One sequence of 131072 keys has 55 parts of a row: eight warps
 /// take every eighth, so that all of them are on their way at once.
 constexpr int kJoinWarps = 8;
-template <int D>
+/// RPB: rows of a block.  One where an item has many parts; eight, a warp each, where it
+/// has a few.
+template <int D, int RPB>
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const ApParams p) {
   pdl_trigger();
   pdl_wait();
   const int4 cut = p.cut[blockIdx.x];
   if (cut.x < 0) return;
-  constexpr int E = D / 32;  // columns of a lane
-  __shared__ float s_o[kJoinWarps][D];
-  __shared__ float s_l[kJoinWarps];
-  const int row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int E = D / 32;            // columns of a lane
+  constexpr int W = kJoinWarps / RPB;  // warps of a row
+  __shared__ float s_o[RPB == 1 ? kJoinWarps : 1][D];
+  __shared__ float s_l[RPB == 1 ? kJoinWarps : 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = blockIdx.y * RPB + warp / W;
   int64_t first;
   const int n_rows = kv_rows(p.c, p.cu, p.seq0 + cut.x, p.n_tokens, &first) * p.group;
-  if (cut.y + row >= n_rows) return;
+  if (cut.y + row >= n_rows) return;  // (whole blocks where RPB is 1)
   const int parts = static_cast<int>(static_cast<unsigned>(cut.z) >> 16);
   const int part0 = 2 * cut.w;
   auto slot = [&](int i) { return static_cast<int64_t>(part0 + (i == 0 ? 1 : 2 * i)) * kPgRows + row; };
@@ -643,7 +676,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
   for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
   float l = 0.0f, o[E] = {};
 #pragma unroll 4
-  for (int i = warp; i < parts; i += kJoinWarps) {
+  for (int i = warp % W; i < parts; i += W) {
     const float2 ml = p.ws_ml[slot(i)];
     float v[E];
     if constexpr (E == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p.ws_o + slot(i) * D + lane * E);
@@ -654,29 +687,36 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = fmaf(v[e], a, o[e]);
   }
+  if constexpr (RPB == 1) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
-  if (lane == 0) s_l[warp] = l;
-  __syncthreads();
-  const int col = threadIdx.x;
-  if (col >= D) return;
-  float sum = 0.0f;
-  l = 0.0f;
+    for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
+    if (lane == 0) s_l[warp] = l;
+    __syncthreads();
+    if (warp != 0) return;
+    l = 0.0f;
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) {
-    sum += s_o[w][col];
-    l += s_l[w];
+    for (int e = 0; e < E; ++e) o[e] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+      l += s_l[w];
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] += s_o[w][lane * E + e];
+    }
   }
   const int64_t at = pg_row(p, first, cut.z & 0xffff, cut.y + row);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  p.out[at * D + col] = __float2half_rn(sum * inv);
-  if (p.lse != nullptr && col == 0)
+  __half2 h[E / 2];
+#pragma unroll
+  for (int e = 0; e < E / 2; ++e) h[e] = __floats2half2_rn(o[2 * e] * inv, o[2 * e + 1] * inv);
+  if constexpr (E == 4) *reinterpret_cast<uint2*>(p.out + at * D + lane * E) = *reinterpret_cast<const uint2*>(h);
+  else *reinterpret_cast<__half2*>(p.out + at * D + lane * E) = h[0];
+  if (p.lse != nullptr && lane == 0)
     p.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
-/// `most`: tiles (items, where p.whole) that there can be.
+/// `most`: steps (items, where p.whole) that there can be; `items`: as it says.
 template <int D, bool E4M3, int NQ>
-int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most, cudaStream_t st) {
+int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most, int64_t items, cudaStream_t st) {
   using Cfg = PgCfg<D, NQ>;
   auto kern = attn_paged_kernel<D, E4M3, NQ>;
   const size_t smem = Cfg::smem(p.n_seq);
@@ -705,7 +745,6 @@ int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most, cudaStre
   const int64_t ctas = std::min<int64_t>(sm_count() * std::max<int64_t>(per_sm, 1), most);
   // One row per sequence: the items are numbered, and the join has a block column for each.
   // Else they are known by the CTA that began them.
-  const int64_t items = static_cast<int64_t>(p.n_seq) * ((p.group + kPgRows - 1) / kPgRows) * p.c.heads;
   p.by_item = p.cu == nullptr && items <= ctas ? 1 : 0;
   const int64_t cuts = p.by_item ? items : ctas;
   const size_t o_bytes = 2 * ctas * kPgRows * D * sizeof(float), ml_bytes = 2 * ctas * kPgRows * sizeof(float2);
@@ -716,9 +755,13 @@ int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most, cudaStre
   p.cut = reinterpret_cast<int4*>(ws + o_bytes + ml_bytes);
   int rc = ENGINE_OK;
   cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPgThreads), smem, st, tk, tv, p);
-  if (e == cudaSuccess)
-    e = launch_pdl(attn_paged_join_kernel<D>, dim3(static_cast<unsigned>(cuts), Cfg::kRows), dim3(kJoinWarps * 32), 0,
-                   st, p);
+  const unsigned c = static_cast<unsigned>(cuts);
+  if (e == cudaSuccess) {
+    if (ctas >= 8 * items)
+      e = launch_pdl(attn_paged_join_kernel<D, 1>, dim3(c, Cfg::kRows), dim3(kJoinWarps * 32), 0, st, p);
+    else
+      e = launch_pdl(attn_paged_join_kernel<D, 8>, dim3(c, Cfg::kRows / 8), dim3(kJoinWarps * 32), 0, st, p);
+  }
   if (e != cudaSuccess) rc = set_cuda_error(e, "attn_paged_kernel");
   scratch_free(ws, st);
   return rc;
@@ -728,6 +771,7 @@ int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most, cudaStre
 int run_paged(ApParams p, const engine_kv_pages_t* kv, int64_t n_seq, cudaStream_t st, const char* what) {
   const bool e4m3 = kv->type == ENGINE_KV_E4M3;
   const int64_t tiles = std::max<int64_t>((kv->max_pages * kv->page_size + kPgKeys - 1) / kPgKeys, 1);
+  const int64_t steps = tiles + kPgItemCost;
   const bool r8 = p.cu == nullptr && p.group <= 8;
   // Rows per sequence and KV head, on the average (the host knows no more).
   const bool many = p.cu != nullptr && p.group <= 128 && p.n_tokens * p.group >= kManyRows * n_seq;
@@ -739,20 +783,20 @@ int run_paged(ApParams p, const engine_kv_pages_t* kv, int64_t n_seq, cudaStream
       if (const int rc = attention_paged_tc(p, kv, st)) return rc;
       continue;
     }
-    // At most this many tiles (the kernel counts them in 32 bits).
+    // At most this many steps (the kernel counts them in 32 bits).
     const int64_t groups = p.cu == nullptr ? n * ((p.group + kPgRows - 1) / kPgRows)
                                            : p.n_tokens * p.group / kPgRows + n;
-    if (groups > 0x7fffffff / kv->n_kv_heads / tiles)
+    if (groups > 0x7fffffff / kv->n_kv_heads / steps)
       return set_error(ENGINE_ERR_UNSUPPORTED, std::string(what) + ": too many query rows x positions");
     p.whole = tiles <= kWholeTiles ? 1 : 0;
-    const int64_t most = groups * kv->n_kv_heads * (p.whole ? 1 : tiles);
+    const int64_t most = groups * kv->n_kv_heads * (p.whole ? 1 : steps);
     int rc;
     if (kv->head_dim == 64) {
-      rc = e4m3 ? (r8 ? launch_paged<64, true, 1>(p, kv, most, st) : launch_paged<64, true, 2>(p, kv, most, st))
-                : (r8 ? launch_paged<64, false, 1>(p, kv, most, st) : launch_paged<64, false, 2>(p, kv, most, st));
+      rc = e4m3 ? (r8 ? launch_paged<64, true, 1>(p, kv, most, groups * kv->n_kv_heads, st) : launch_paged<64, true, 2>(p, kv, most, groups * kv->n_kv_heads, st))
+                : (r8 ? launch_paged<64, false, 1>(p, kv, most, groups * kv->n_kv_heads, st) : launch_paged<64, false, 2>(p, kv, most, groups * kv->n_kv_heads, st));
     } else {
-      rc = e4m3 ? (r8 ? launch_paged<128, true, 1>(p, kv, most, st) : launch_paged<128, true, 2>(p, kv, most, st))
-                : (r8 ? launch_paged<128, false, 1>(p, kv, most, st) : launch_paged<128, false, 2>(p, kv, most, st));
+      rc = e4m3 ? (r8 ? launch_paged<128, true, 1>(p, kv, most, groups * kv->n_kv_heads, st) : launch_paged<128, true, 2>(p, kv, most, groups * kv->n_kv_heads, st))
+                : (r8 ? launch_paged<128, false, 1>(p, kv, most, groups * kv->n_kv_heads, st) : launch_paged<128, false, 2>(p, kv, most, groups * kv->n_kv_heads, st));
     }
     if (rc != ENGINE_OK) return rc;
   }
