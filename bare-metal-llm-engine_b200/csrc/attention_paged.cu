@@ -727,6 +727,7 @@ int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most, int64_t 
   if ((configured.load() & bit) == 0) {
     B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    static_cast<int>(Cfg::smem(kPgMaxSeq))));
+    B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     configured.fetch_or(bit);
   }
   CUtensorMap tk, tv;
@@ -754,7 +755,11 @@ int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most, int64_t 
   p.ws_ml = reinterpret_cast<float2*>(ws + o_bytes);
   p.cut = reinterpret_cast<int4*>(ws + o_bytes + ml_bytes);
   int rc = ENGINE_OK;
-  cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPgThreads), smem, st, tk, tv, p);
+  // A plain launch: an SM that still runs blocks of the kernel before keeps their split of its
+  // storage, and begun under it takes two of these CTAs where it should take three; the shares
+  // left over then begin when the others are done (85 us against 71 for the call).
+  kern<<<static_cast<unsigned>(ctas), kPgThreads, smem, st>>>(tk, tv, p);
+  cudaError_t e = cudaGetLastError();
   const unsigned c = static_cast<unsigned>(cuts);
   if (e == cudaSuccess) {
     if (ctas >= 8 * items)
