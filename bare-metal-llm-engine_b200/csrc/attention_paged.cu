@@ -48,7 +48,7 @@ constexpr float kPgRescale = 8.0f;
 /// What an item costs beside its key tiles (its q, the chain of its first tile, the join of
 /// the warps), in tiles: the even shares count it, as steps in front of the item's tiles in
 /// which nothing is done.
-constexpr int kPgItemCost = 3;
+constexpr int kPgItemCost = 4;
 constexpr int64_t kManyRows = 32;  // from here on attention_paged_tc
 constexpr int64_t kWholeTiles = 16;  // slots of at most so many tiles: a CTA to an item
 static_assert(kPgMaxSeq <= kTcMaxSeq, "both kernels take a launch's sequences");

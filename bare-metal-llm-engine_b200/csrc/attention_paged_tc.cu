@@ -73,6 +73,7 @@ struct TcItem {
   int head, qb;
   int t0, t1, tiles;
   int begin;  // the item's first step, counted over all items
+  bool two;   // side B has rows
 };
 
 __device__ __forceinline__ int tc_tiles(const TcParams& p, int len, int n_tok, int qb) {
@@ -90,7 +91,8 @@ __device__ __forceinline__ void tc_sequence(const TcParams& p, int b, TcItem& it
 }
 
 /// The tiles that the steps from x on, before hi, have of the item.
-__device__ __forceinline__ void tc_range(TcItem& it, int x, int hi) {
+__device__ __forceinline__ void tc_range(const TcParams& p, TcItem& it, int x, int hi) {
+  it.two = (it.qb * 2 + 1) * p.tq < it.n_tok;
   it.t0 = max(x - it.begin - kTcItemCost, 0);
   it.t1 = max(min(hi - it.begin - kTcItemCost, it.tiles), it.t0);
 }
@@ -110,7 +112,7 @@ __device__ __forceinline__ void tc_next(const TcParams& p, TcItem& it, int x, in
   }
   it.begin = x;
   it.tiles = tc_tiles(p, it.len, it.n_tok, it.qb);
-  tc_range(it, x, hi);
+  tc_range(p, it, x, hi);
 }
 
 /// The item at step x, found by the whole warp.  pre: steps before each sequence.
@@ -146,7 +148,7 @@ __device__ TcItem tc_find(const TcParams& p, const int32_t* pre, int x, int hi) 
     }
     z -= __shfl_sync(0xffffffffu, incl, 31);
   }
-  tc_range(it, x, hi);
+  tc_range(p, it, x, hi);
   return it;
 }
 
@@ -447,7 +449,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int g = lane >> 2, t4 = lane & 3;
     const uint32_t tS = tmem + (static_cast<uint32_t>(r0) << 16) + side * 128;
     const uint32_t tO = tmem + (static_cast<uint32_t>(r0) << 16) + Cfg::kColO + side * D;
-    int n = 0;
+    int n = 0, nb = 0;  // tiles, and those that B had a part in
     bool ok = true;
     // Token within the side's, or far past any, and head within the group of the thread's rows.
     int q_tok[2], q_head[2];
@@ -458,16 +460,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       q_head[r] = q % p.a.group;
     }
     for (int x = lo; x < hi && ok && it.t0 < it.t1;) {
+      if (side == 1 && !it.two) {
+        n += it.t1 - it.t0;
+        x = tc_end(it);
+        if (x < hi) tc_next(p, it, x, hi);
+        continue;
+      }
       const int left = it.n_tok - (it.qb * 2 + side) * p.tq;  // tokens of the sequence from the side's first on
       int lim[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r)
         lim[r] = p.a.causal && q_tok[r] < left ? it.len - left + q_tok[r] + 1 : it.len;
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-      for (int t = it.t0; t < it.t1; ++t, ++n) {
+      for (int t = it.t0; t < it.t1; ++t, ++n, nb += it.two ? 1 : 0) {
         const float4* con = s_const + (n & 3) * 8;
         const int key = t * kTcKeys + 2 * t4;
-        ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->s_full[side], n & 1, limit, c.err));
+        ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->s_full[side], (side ? nb : n) & 1, limit, c.err));
         if (!ok) break;
         tc_fence_after();
         const bool clean =
@@ -509,8 +517,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         // The sides' exponentials take turns: A after B's last tile, B after A's this one.  In
         // step, both would want them at once and both would then want the tensor cores.
-        if (side == 1 || n > 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->p_full[side ^ 1][1], side ? n & 1 : (n - 1) & 1,
+        // (A waits in items without a side B too, so that it is never two tiles ahead of B's wait.)
+        if (side == 1 || nb > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->p_full[side ^ 1][1], side ? n & 1 : (nb - 1) & 1,
                                                         limit, c.err));
           if (!ok) break;
         }
@@ -532,7 +541,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
       }
-      ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->o_done[side], (n - 1) & 1, limit, c.err));
+      ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->o_done[side], ((side ? nb : n) - 1) & 1, limit, c.err));
       if (!ok) break;
       tc_fence_after();
       const bool whole = it.t1 - it.t0 == it.tiles;
@@ -672,17 +681,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint64_t dk = umma_desc_sw128(smem_u32(smem + Cfg::kOffK), 16, 1024);
       const uint64_t dv = umma_desc_sw128(smem_u32(smem + Cfg::kOffV), 8192, 1024);
       const uint32_t tS = tmem + side * 128, tO = tmem + Cfg::kColO + side * D;
-      int n = 0, items = 0;
+      int n = 0;           // tiles
+      int mine = 0;        // tiles of this side
+      int items = 0, own = 0;  // items, and this side's
       bool ok = true;
       bool busy = false;  // something was issued
-      auto pv = [&](int i, bool start) {  // O += P V of tile i; `start`: the item's first
+      auto pv = [&](int i, bool start) {  // O += P V of tile i, this side's last one; `start`: the item's first
         ok = mbar_wait(&bar->v_full[i & 1], (i >> 1) & 1, limit, c.err);
         // It overwrites O: the last item's rows have been read.
-        if (ok && start) ok = mbar_wait(&bar->o_free[side], (items & 1) ^ 1u, limit, c.err);
+        if (ok && start) ok = mbar_wait(&bar->o_free[side], (own & 1) ^ 1u, limit, c.err);
         const uint64_t d = dv + static_cast<uint64_t>((i & 1) * (Cfg::kWide >> 4));
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          if (ok) ok = mbar_wait(&bar->p_full[side][half], i & 1, limit, c.err);
+          if (ok) ok = mbar_wait(&bar->p_full[side][half], (mine - 1) & 1, limit, c.err);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) return;
           tc_fence_after();
@@ -702,30 +713,48 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       };
       for (int x = lo; x < hi && ok && it.t0 < it.t1; ++items) {
         ok = mbar_wait(&bar->q_full, items & 1, limit, c.err);
-        for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
-          ok = mbar_wait(&bar->k_full[n & 1], (n >> 1) & 1, limit, c.err);
-          if (ok && t > it.t0) pv(n - 1, t == it.t0 + 1);
-          // S goes over P of the tile before: its product must have read it.
-          if (ok && n > 0) ok = mbar_wait(&bar->o_done[side], (n - 1) & 1, limit, c.err);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
-          if (leader) {
-            const uint64_t d = dk + static_cast<uint64_t>((n & 1) * (Cfg::kWide >> 4));
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              umma_f16(tS, dq + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
-                       d + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), kIdescS, kk > 0 ? 1u : 0u);
-            umma_commit(&bar->s_full[side]);
-            umma_commit(&bar->k_empty[n & 1]);
+        if (side == 1 && !it.two) {
+          // No rows here: the tiles are only given back.
+          for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
+            ok = mbar_wait(&bar->k_full[n & 1], (n >> 1) & 1, limit, c.err);
+            if (ok) ok = mbar_wait(&bar->v_full[n & 1], (n >> 1) & 1, limit, c.err);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok && leader) {
+              mbar_arrive(&bar->k_empty[n & 1]);
+              mbar_arrive(&bar->v_empty[n & 1]);
+            }
+            __syncwarp();
           }
+          if (ok && leader) mbar_arrive(&bar->q_empty);
           __syncwarp();
-          busy = true;
+        } else {
+          for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
+            ok = mbar_wait(&bar->k_full[n & 1], (n >> 1) & 1, limit, c.err);
+            if (ok && t > it.t0) pv(n - 1, t == it.t0 + 1);
+            // S goes over P of the tile before: its product must have read it.
+            if (ok && mine > 0) ok = mbar_wait(&bar->o_done[side], (mine - 1) & 1, limit, c.err);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            if (leader) {
+              const uint64_t d = dk + static_cast<uint64_t>((n & 1) * (Cfg::kWide >> 4));
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk)
+                umma_f16(tS, dq + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
+                         d + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), kIdescS, kk > 0 ? 1u : 0u);
+              umma_commit(&bar->s_full[side]);
+              umma_commit(&bar->k_empty[n & 1]);
+            }
+            __syncwarp();
+            busy = true;
+            ++mine;
+          }
+          if (!ok) break;
+          if (leader) umma_commit(&bar->q_empty);
+          __syncwarp();
+          pv(n - 1, it.t1 - it.t0 == 1);
+          ++own;
         }
-        if (!ok) break;
-        if (leader) umma_commit(&bar->q_empty);
-        __syncwarp();
-        pv(n - 1, it.t1 - it.t0 == 1);
         x = tc_end(it);
         if (x < hi) tc_next(p, it, x, hi);
       }
