@@ -481,12 +481,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const bool clean =
             __all_sync(0xffffffffu, (t + 1) * kTcKeys <= min(lim[0], lim[1]) && con[0].w == 2.0f);
         float mt[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t v[32];
-          tc_half_load<KG>(tS + half * 64, con + half * 4, key + half * 64, lim, clean, v);
-          tc_half_max<KG>(v, con + half * 4, clean, mt);
-        }
+        // The maxima of both halves; the first stays in registers for its weights (with the second
+        // that would be 64, more than a thread has beside the rest).
+        uint32_t v[32];
+        tc_half_load<KG>(tS + 64, con + 4, key + 64, lim, clean, v);
+        tc_half_max<KG>(v, con + 4, clean, mt);
+        tc_half_load<KG>(tS, con, key, lim, clean, v);
+        tc_half_max<KG>(v, con, clean, mt);
         // The rows keep their references until a maximum passes them by 2^14; only then do
         // the four threads of a row compare theirs, and O is rescaled.
         if (__any_sync(0xffffffffu, mt[0] > m[0] + kTcRescale || mt[1] > m[1] + kTcRescale)) {
@@ -525,8 +526,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          uint32_t v[32], pk[16];
-          tc_half_load<KG>(tS + half * 64, con + half * 4, key + half * 64, lim, clean, v);
+          uint32_t pk[16];
+          if (half == 1) tc_half_load<KG>(tS + 64, con + 4, key + 64, lim, clean, v);
           tc_half_weights<KG>(v, con + half * 4, clean, m, l, pk);
           __syncwarp();
           tmem_st_16x128b_x8(tS + half * 32, pk);  // over columns that have been read
