@@ -357,6 +357,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
       float init[NQ][2];
       int lim[NQ][2];
       int least = it.len;
+      uint4 qw[NQ][NK / 2];
 #pragma unroll
       for (int nq = 0; nq < NQ; ++nq) {
         const int flat = it.row0 + 8 * nq + g;
@@ -364,11 +365,15 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
         const uint4* src = reinterpret_cast<const uint4*>(
             p.q + (it.first + (row ? flat / p.group : 0)) * p.q_pitch +
             static_cast<int64_t>(it.head * p.group + (row ? flat % p.group : 0)) * D + t * (D / 4));
+#pragma unroll
+        for (int i = 0; i < NK / 2; ++i) qw[nq][i] = row ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int nq = 0; nq < NQ; ++nq) {
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < NK / 2; ++i) {
-          const uint4 w = row ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
-          const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+          const uint32_t q[4] = {qw[nq][i].x, qw[nq][i].y, qw[nq][i].z, qw[nq][i].w};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             uint32_t u0 = q[2 * e], u1 = q[2 * e + 1];
