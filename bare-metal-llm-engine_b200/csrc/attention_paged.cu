@@ -29,6 +29,13 @@
 // loaded into A fragments in registers.  The order of the contraction is free, so they
 // are consecutive bytes: D / 4 of two keys' rows for S^T, D / 8 of four keys' rows for
 // O^T; P passes from one layout to the other by two 8 x 8 transpositions.
+//   Measured (B200, 32 / 8 heads of 128, calls back to back): 131072 keys of one sequence
+// 55 us (269 MB, 0.75 of the measured copy rate), 48 sequences of 200-16384 keys 72 us (372
+// MB, 0.79), 64 x 4000 keys 94 us (0.85).  Within the kernel the tiles arrive at about 7 TB/s;
+// the rest is the 5 us until the first tile is there (lengths, table, scales and codes, each
+// looked up with the last), the spread of the shares' ends and the join (4 us).  With q as A
+// and the int8 offset taken off every code the first was 66 us where it is 54 to 55.  Eight
+// consumer warps a CTA, two CTAs: 96 registers, spills, 83.
 
 #include <algorithm>
 #include <atomic>
@@ -46,11 +53,19 @@ constexpr int kPgThreads = (kPgConsumers + 1) * 32;
 constexpr int kPgMaxSeq = 1024;  // sequences per launch (their prefix sums sit in shared memory)
 constexpr float kPgRescale = 8.0f;
 /// What an item costs beside its key tiles (its q, the chain of its first tile, the join of
-/// the warps), in tiles: the even shares count it, as steps in front of the item's tiles in
-/// which nothing is done.
+/// the warps: about 4 us against 1 a tile), in tiles: the even shares count it, as steps in
+/// front of the item's tiles in which nothing is done.  48 sequences of 200-16384 keys: 75 us
+/// with 2, 72 with 4, 74 with 8.
 constexpr int kPgItemCost = 4;
-constexpr int64_t kManyRows = 32;  // from here on attention_paged_tc
-constexpr int64_t kWholeTiles = 16;  // slots of at most so many tiles: a CTA to an item
+/// Query rows of a sequence and KV head (the average: the host knows no more) from which
+/// attention_paged_tc takes the call.  One sequence of 4000 keys: 24 rows 25 us either way, 32
+/// rows 23 us there and 27 here, 64 rows 23 and 29; sixteen of them: 16 rows 83 and 50, 32
+/// rows 80 and 77, 48 rows 82 and 103.
+constexpr int64_t kManyRows = 32;
+/// Slots of at most so many tiles have a CTA to an item: no workspace, no join.  1000 keys: one
+/// sequence 13 us and 16 split, 8 sequences 14 and 16, 256 sequences 102 and 103; at 2000 keys
+/// (32 tiles) it would be 21 and 16, 26 and 20, 176 and 179.
+constexpr int64_t kWholeTiles = 16;
 static_assert(kPgMaxSeq <= kTcMaxSeq, "both kernels take a launch's sequences");
 
 /// NQ: groups of 8 query rows of an item.  Three CTAs an SM with 128 registers a thread

@@ -183,7 +183,8 @@ __device__ __forceinline__ uint2 wr_codes(const uint4& x, float inv) {
 
 // Several rows: a CTA takes kWrTiles (KV head, K | V) tiles of one page, one after the
 // other with the next one's rows on their way, so that finding the page (three dependent
-// lookups) is paid once for them.
+// lookups) is paid once for them.  (Tiles one by one 21 us, two 20.8, four 19.3, eight 18.9
+// but fewer CTAs for short prompts.)
 constexpr int kWrTiles = 4;
 
 template <int PASSES, bool E4M3>

@@ -231,6 +231,57 @@ inline void kv_cache_write(const __half* k_new, const __half* v_new, __half* k_c
 }  // namespace detail
 #endif  // ENGINE_B200_NO_ATTENTION
 
+// -- paged 8-bit KV cache (engine_kv_pages_t, engine_b200.h) --------------------
+// No counterpart in kernels.hpp.  A view of the caller's device memory, filled in by
+// hand; the functions check it on every call.  Statuses are device words: read them
+// when they are wanted.
+using KvPages = engine_kv_pages_t;
+
+inline void kv_pages_extend(const KvPages& kv, const std::int32_t* slots, const std::int32_t* n_new,
+                            std::int32_t* status, std::int64_t n, cudaStream_t stream = 0) {
+  b200_detail::check(engine_cuda_kv_pages_extend(&kv, slots, n_new, status, n, stream));
+}
+inline void kv_pages_fork(const KvPages& kv, const std::int32_t* parents,
+                          const std::int32_t* children, std::int32_t* status, std::int64_t n,
+                          cudaStream_t stream = 0) {
+  b200_detail::check(engine_cuda_kv_pages_fork(&kv, parents, children, status, n, stream));
+}
+inline void kv_pages_free(const KvPages& kv, const std::int32_t* slots, std::int64_t n,
+                          cudaStream_t stream = 0) {
+  b200_detail::check(engine_cuda_kv_pages_free(&kv, slots, n, stream));
+}
+inline void kv_pages_compact(const KvPages& kv, std::int32_t* remap = nullptr,
+                             cudaStream_t stream = 0) {
+  b200_detail::check(engine_cuda_kv_pages_compact(&kv, remap, stream));
+}
+// cu_new null: one row per sequence, n_tokens = n_seq.
+inline void kv_pages_write(const KvPages& kv, std::int64_t layer, const __half* k_new,
+                           const __half* v_new, std::int64_t row_pitch, const std::int32_t* slots,
+                           const std::int32_t* cu_new, std::int64_t n_seq, std::int64_t n_tokens,
+                           cudaStream_t stream = 0) {
+  b200_detail::check(engine_cuda_kv_pages_write(&kv, layer, b200_detail::h(k_new),
+                                                b200_detail::h(v_new), row_pitch, slots, cu_new,
+                                                n_seq, n_tokens, stream));
+}
+inline void attention_paged_decode(const KvPages& kv, std::int64_t layer, const __half* q,
+                                   std::int64_t q_pitch, const std::int32_t* slots, __half* out,
+                                   std::int64_t n_seq, std::int64_t n_heads, float scale,
+                                   float* out_lse = nullptr, cudaStream_t stream = 0) {
+  b200_detail::check(engine_cuda_attention_paged_decode(&kv, layer, b200_detail::h(q), q_pitch,
+                                                        slots, b200_detail::h(out), out_lse, n_seq,
+                                                        n_heads, scale, stream));
+}
+inline void attention_paged_prefill(const KvPages& kv, std::int64_t layer, const __half* q,
+                                    std::int64_t q_pitch, const std::int32_t* slots,
+                                    const std::int32_t* cu_q, __half* out, std::int64_t n_seq,
+                                    std::int64_t n_tokens, std::int64_t n_heads, float scale,
+                                    bool is_causal = true, float* out_lse = nullptr,
+                                    cudaStream_t stream = 0) {
+  b200_detail::check(engine_cuda_attention_paged_prefill(
+      &kv, layer, b200_detail::h(q), q_pitch, slots, cu_q, b200_detail::h(out), out_lse, n_seq,
+      n_tokens, n_heads, scale, is_causal ? 1 : 0, stream));
+}
+
 // -- tensor-parallel communicator (engine_tp_*) --------------------------------
 // One per rank, on the rank's current device.  The host exchanges handle()
 // between the ranks (all-gather), then calls open() with all of them in rank

@@ -33,7 +33,11 @@
  *     engine_cuda_attention_decode / _prefill with split partials to merge (the
  *     tcgen05 decode with more than 8 splits per KV head, or the CUDA-core
  *     kernels with more than one; up to 8 tcgen05 splits merge inside a
- *     thread-block cluster and need none);
+ *     thread-block cluster and need none),
+ *     engine_cuda_attention_paged_decode / _prefill (the parts of sequences that
+ *     are split over CTAs: at most 8 MB, 39 MB with more than 32 query rows per
+ *     sequence and KV head; none for slots of at most 1024 positions) and
+ *     engine_cuda_kv_pages_fork / _compact (a few words per slot or page);
  *   - once per (device, stream), on the first call that needs it, never during
  *     a stream capture: the stream-K workspace of the large 16-bit GEMMs
  *     (engine_cuda_matmul_* / linear_* with M, N >= 256; about 38 MB);
@@ -462,8 +466,9 @@ ENGINE_B200_API int engine_cuda_kv_pages_compact(const engine_kv_pages_t* kv, in
  * codes q become round(q * (old / new)).  A new row's codes are round(x * (1 / scale))
  * (0 for scale 0).  An infinity or NaN cannot be held in 8 bits: the scale
  * becomes NaN, so that attention to that (page, head) answers NaN.
- *   Pages written to must have one user.  k_new, v_new 16-byte aligned, row_pitch
- * a multiple of 8. */
+ *   Pages written to must have one user (extend and fork see to that), and a slot
+ * occurs once in a call.  k_new, v_new 16-byte aligned, row_pitch a multiple of 8
+ * (ENGINE_ERR_UNSUPPORTED otherwise). */
 ENGINE_B200_API int engine_cuda_kv_pages_write(const engine_kv_pages_t* kv, int64_t layer,
                                                const engine_half_t* k_new,
                                                const engine_half_t* v_new, int64_t row_pitch,
@@ -476,7 +481,7 @@ ENGINE_B200_API int engine_cuda_kv_pages_write(const engine_kv_pages_t* kv, int6
  * its slot.  q row i at i * q_pitch elements, [n_heads][head_dim]; out
  * [n_seq][n_heads][head_dim] and out_lse [n_seq][n_heads] (natural log, may be
  * null) contiguous.  An empty slot gives zeros and -inf.  q and out 16-byte
- * aligned, q_pitch a multiple of 8. */
+ * aligned, q_pitch a multiple of 8, scale positive. */
 ENGINE_B200_API int engine_cuda_attention_paged_decode(const engine_kv_pages_t* kv, int64_t layer,
                                                        const engine_half_t* q, int64_t q_pitch,
                                                        const int32_t* slots, engine_half_t* out,

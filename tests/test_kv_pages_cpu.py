@@ -110,6 +110,54 @@ def test_paged_kv_checks_its_tensors(pkg):
         pkg.ops.PagedKV(**{**good, "k": good["k"][0], "v": good["v"][0]})
 
 
+def test_cpp_adapter(pkg, tmp_path):
+    """engine::cuda::kv_pages_* / attention_paged_* of kernels_b200.hpp: they compile, link,
+    and throw EngineError with the library's message before any device work."""
+    import subprocess
+
+    src = r"""
+#include <cstdio>
+#include <engine/kernels_b200.hpp>
+namespace ec = engine::cuda;
+template <typename F> static int throws(F f, const char* part) {
+  try { f(); } catch (const engine::EngineError& e) {
+    if (std::string(e.what()).find(part) != std::string::npos) return 0;
+    std::printf("%s\n", e.what());
+  }
+  return 1;
+}
+int main() {
+  ec::KvPages kv = {};
+  auto* p = reinterpret_cast<void*>(4096);
+  auto* i = reinterpret_cast<std::int32_t*>(4096);
+  auto* h = reinterpret_cast<__half*>(4096);
+  int bad = throws([&] { ec::kv_pages_compact(kv); }, "k/v is null");
+  kv.k = kv.v = p;
+  kv.k_scale = kv.v_scale = reinterpret_cast<float*>(p);
+  kv.table = kv.length = kv.ref = i;
+  kv.n_layers = 1; kv.n_pages = 4; kv.n_kv_heads = 2; kv.page_size = 16; kv.head_dim = 64;
+  kv.n_slots = 2; kv.max_pages = 2; kv.type = ENGINE_KV_E4M3;
+  bad += throws([&] { ec::kv_pages_extend(kv, i, i, nullptr, 1); }, "status is null");
+  bad += throws([&] { ec::kv_pages_fork(kv, i, nullptr, i, 1); }, "children is null");
+  bad += throws([&] { ec::kv_pages_free(kv, i, -1); }, "non-negative");
+  bad += throws([&] { ec::kv_pages_write(kv, 1, h, h, 128, i, i, 1, 1); }, "layer out of range");
+  bad += throws([&] { ec::attention_paged_decode(kv, 0, h, 256, i, h, 1, 3, 0.125f); }, "divisible");
+  bad += throws([&] { ec::attention_paged_prefill(kv, 0, h, 256, i, nullptr, h, 1, 1, 4, 0.125f); }, "cu_q is null");
+  return bad;
+}
+"""
+    from tests.conftest import ROOT
+
+    exe = tmp_path / "kv_pages"
+    (tmp_path / "kv_pages.cpp").write_text(src)
+    r = subprocess.run(["g++", "-std=c++17", f"-I{ROOT / 'include'}", "-I/usr/local/cuda/include",
+                        str(tmp_path / "kv_pages.cpp"), "-o", str(exe), str(pkg.LIB_PATH),
+                        f"-Wl,-rpath,{pkg.LIB_PATH.parent}"], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout
+
+
 def test_calls_check_their_tensors(pkg, monkeypatch):
     """Another current device, other types, shapes and strides: refused in Python, with a
     stand-in for the cache (nothing reaches the library)."""
