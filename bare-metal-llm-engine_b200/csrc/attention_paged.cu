@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
         if (n == 0) {
           for (; ahead < min(count, ST) && ok; ++ahead) fetch(ahead, ahead);
         }
-        const float v1 = vs == 0.0f ? 1.0f : vs;
+        const float v1 = vs == 0.0f ? kNoScale : vs;
         const float4 con = id >= 0 ? make_float4(ks * kc_unit, log2f(v1), 1.0f / v1, 1.0f)
                                    : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
         int id2 = -1;

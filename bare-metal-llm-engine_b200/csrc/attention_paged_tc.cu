@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (id >= 0) {
             const float ks = c.ks[kv_scale_at(c, id, it.head)];
             float vs = c.vs[kv_scale_at(c, id, it.head)];
-            if (vs == 0.0f) vs = 1.0f;
+            if (vs == 0.0f) vs = kNoScale;
             con = make_float4(ks * p.a.scale_log2, log2f(vs), 1.0f / vs, 1.0f);
           }
           const unsigned valid = __ballot_sync(0xffffffffu, id >= 0);

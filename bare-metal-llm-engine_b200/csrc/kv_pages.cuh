@@ -31,6 +31,10 @@ struct KvView {
 
 constexpr float kQMaxI8 = 127.0f;
 constexpr float kQMaxE4M3 = 448.0f;
+/// What attention takes for a scale of V that is 0 (a page of zeros, whose weights count in
+/// the denominator alone): below any that a write gives, so that w = p vs of such a page is
+/// never what the others' weights are rounded against.
+constexpr float kNoScale = 1.1641532182693481e-10f;  // 2^-33 < 2^-24 / 448
 
 /// Validates the descriptor (and `layer`, unless it is -1: all layers); returns
 /// ENGINE_OK or an error with the message recorded.  kv_pages.cu.

@@ -278,6 +278,30 @@ def test_prefill(pkg, dev, dtype, heads, hk, d, page, causal):
     assert pkg.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [I8, E4M3])
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_pages_of_zeros_beside_small_values(pkg, dev, dtype, new):
+    """A key in a page whose V is all zeros takes most of the weight, beside values of about
+    1e-3: the others' weights keep their precision."""
+    hk, d, page = 2, 64, 16
+    m, kv = make(pkg, dev, hk=hk, d=d, page=page, dtype=dtype)
+    n = 5 * page
+    assert int(pkg.ops.kv_pages_extend(kv, i32([0], dev), i32([n], dev))) == m.extend([0], [n]) == 0
+    g = torch.Generator().manual_seed(8)
+    q = (1 + 0.1 * torch.randn(new, 4, d, generator=g)).half().to(dev)
+    k = 0.05 * torch.randn(n, hk * d, generator=g)
+    k[0] = 0.52  # a score 4.2 above the others'
+    v = 1e-3 * torch.randn(n, hk * d, generator=g)
+    v[:page] = 0
+    v[2 * page:3 * page] = 0
+    pkg.ops.kv_pages_write(kv, 0, k.half().to(dev), v.half().to(dev), i32([0], dev), i32([0, n], dev))
+    if new == 1:
+        out, lse = pkg.ops.attention_paged_decode(kv, 0, q, i32([0], dev), want_lse=True)
+    else:
+        out, lse = pkg.ops.attention_paged_prefill(kv, 0, q, i32([0], dev), i32([0, new], dev), want_lse=True)
+    ref.check_attention(kv, 0, q, out, [0], [0, new], d ** -0.5, True, lse)
+
+
 def test_prefill_rows_that_see_nothing(pkg, dev):
     """More query rows than positions: the first rows see no key."""
     m, kv = make(pkg, dev, hk=2, d=128, page=16)
