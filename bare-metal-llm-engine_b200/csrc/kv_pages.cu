@@ -414,6 +414,8 @@ __global__ void __launch_bounds__(kBkThreads) kv_extend_kernel(const BkParams p)
   pdl_wait();
   __shared__ int s_start[ENGINE_KV_MAX_SLOTS];
   __shared__ int s_len[ENGINE_KV_MAX_SLOTS];  // length before; -1 where not claimed here
+  __shared__ unsigned long long s_need;       // pages, which may be more than 32 bits hold
+  if (threadIdx.x == 0) s_need = 0;
   const int64_t cap = p.max_pages << p.shift;
   const int page = 1 << p.shift;
   bool bad = false;
@@ -436,11 +438,18 @@ __global__ void __launch_bounds__(kBkThreads) kv_extend_kernel(const BkParams p)
   bad = __syncthreads_or(bad);
   int missing = 0;
   if (!bad) {
-    const int want = sum_needs(p.n, s_start, [&](int i) {
+    auto need = [&](int i) {
       return ((s_len[i] + p.b[i] + page - 1) >> p.shift) - ((s_len[i] + page - 1) >> p.shift);
-    });
+    };
+    unsigned long long mine = 0;
+    for (int i = threadIdx.x; i < p.n; i += kBkThreads) mine += need(i);
+    if (mine != 0) atomicAdd(&s_need, mine);
+    __syncthreads();
+    const int64_t all = static_cast<int64_t>(s_need);
+    const int want = static_cast<int>(min(all, p.n_pages + 1));  // enough to count them all
     const int have = for_free_pages(p, want, [](int, int32_t) {});
-    missing = want > have ? want - have : 0;
+    if (all > have) missing = static_cast<int>(min(all - have, static_cast<int64_t>(0x7fffffff)));
+    else sum_needs(p.n, s_start, need);
     if (missing == 0) {
       for_free_pages(p, want, [&](int rank, int32_t id) {
         const int i = owner_of(s_start, p.n, rank);

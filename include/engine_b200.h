@@ -427,8 +427,8 @@ typedef struct {
 
 /* length[slots[i]] += n_new[i], taking the pages that this needs from the free
  * ones, lowest id first, in the order of i and then of position.  All or
- * nothing: *status (device) = 0, or the number of pages that were missing, or
- * -1 (and error bit 2) for a slot out of range or named twice, a negative n_new
+ * nothing: *status (device) = 0, or the number of pages that were missing (at
+ * most 2^31 - 1), or -1 (and error bit 2) for a slot out of range or named twice, a negative n_new
  * or a row too short; unless 0, nothing changed. */
 ENGINE_B200_API int engine_cuda_kv_pages_extend(const engine_kv_pages_t* kv, const int32_t* slots,
                                                 const int32_t* n_new, int32_t* status, int64_t n,

@@ -203,6 +203,20 @@ def test_refused_calls_change_nothing(pkg, dev):
     assert pkg.device_status() == 0
 
 
+def test_extend_by_more_pages_than_32_bits_count(pkg, dev):
+    """2048 slots that want 2^20 pages each: refused, with the number that is missing."""
+    n, per = 2048, 2 ** 20
+    kv = pkg.ops.PagedKV.empty(1, 40, 1, 16, 64, n, per, I8, dev)  # 8.6 GB of table
+    st = pkg.ops.kv_pages_extend(kv, None, i32([per * 16] * n, dev))
+    assert int(st) == 2 ** 31 - 40 and kv.length.eq(0).all() and kv.ref.eq(0).all()
+    st = pkg.ops.kv_pages_extend(kv, i32([3, 9], dev), i32([17, 600], dev))
+    assert int(st) == 0 and kv.ref.sum() == 40
+    st = pkg.ops.kv_pages_extend(kv, None, i32([16] * n, dev))
+    assert int(st) == n
+    assert kv.table[9, :38].tolist() == list(range(2, 40)) and kv.length.sum() == 617
+    assert pkg.device_status() == 0
+
+
 def test_many_slots_and_pages(pkg, dev):
     """The most slots of a call, and pools of several thousand pages."""
     n = 2048
