@@ -237,19 +237,21 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
   }
   __syncthreads();
   if (warp == 0) {
-    int run = 0;
+    unsigned run = 0;
+    int64_t all = 0;
     for (int base = 0; base < p.n_seq; base += 32) {
       const int v = base + lane < p.n_seq ? s_pre[base + lane] : 0;
-      int incl = v;
+      unsigned incl = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        const unsigned u = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += u;
       }
-      if (base + lane < p.n_seq) s_pre[base + lane] = run + incl - v;
+      if (base + lane < p.n_seq) s_pre[base + lane] = static_cast<int>(run + incl - v);
       run += __shfl_sync(0xffffffffu, incl, 31);
+      all += kv_wide_sum(v);
     }
-    if (lane == 0) s_pre[p.n_seq] = run;
+    if (lane == 0) s_pre[p.n_seq] = kv_total(p.c, all);
   }
   __syncthreads();
   const PgLists lists{s_pre, s_slot, s_len};

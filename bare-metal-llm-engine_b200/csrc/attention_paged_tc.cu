@@ -356,19 +356,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
   __syncthreads();
   if (warp == 0) {
-    int run = 0;
+    unsigned run = 0;
+    int64_t all = 0;
     for (int base = 0; base < p.a.n_seq; base += 32) {
       const int v = base + lane < p.a.n_seq ? s_pre[base + lane] : 0;
-      int incl = v;
+      unsigned incl = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        const unsigned u = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += u;
       }
-      if (base + lane < p.a.n_seq) s_pre[base + lane] = run + incl - v;
+      if (base + lane < p.a.n_seq) s_pre[base + lane] = static_cast<int>(run + incl - v);
       run += __shfl_sync(0xffffffffu, incl, 31);
+      all += kv_wide_sum(v);
     }
-    if (lane == 0) s_pre[p.a.n_seq] = run;
+    if (lane == 0) s_pre[p.a.n_seq] = kv_total(c, all);
   }
   __syncthreads();
   const int total = s_pre[p.a.n_seq];

@@ -90,6 +90,19 @@ __device__ __forceinline__ int kv_rows(const KvView& c, const int32_t* cu, int64
   return e - a;
 }
 
+/// Sum of v >= 0 over the warp, which may pass 32 bits.
+__device__ __forceinline__ int64_t kv_wide_sum(int v) {
+  return (static_cast<int64_t>(__reduce_add_sync(0xffffffffu, v >> 16)) << 16) +
+         __reduce_add_sync(0xffffffffu, v & 0xffff);
+}
+/// Steps of a launch from their exact sum.  The host has bounded those of sequences that share
+/// no rows; entries of cu that go back and forth can pass 32 bits: nothing is done then.
+__device__ __forceinline__ int kv_total(const KvView& c, int64_t all) {
+  if (all <= 0x7fffffff) return static_cast<int>(all);
+  atomicOr(c.err, kErrBadArgument);
+  return 0;
+}
+
 /// First code of (page, head, row 0) for head_dim D, and the index of its scale.
 template <int D>
 __device__ __forceinline__ int64_t kv_tile(const KvView& c, int page, int head) {

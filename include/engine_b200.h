@@ -398,8 +398,9 @@ ENGINE_B200_API int engine_cuda_rmsnorm_linear_kv_f16(
  * All of it is device memory that the kernels read, so the calls need no host
  * synchronisation and can be captured; calls that use one cache are ordered by
  * the caller (one stream, or events).  Entries that are out of range -- a slot
- * outside [0, n_slots), a length beyond the row, a page id outside [0, n_pages)
- * -- set error bit 2 (engine_device_status) and are left out.
+ * outside [0, n_slots), a length beyond the row, a page id outside [0, n_pages),
+ * rows (cu_new, cu_q) that are no ascending pair within n_tokens -- set error bit
+ * 2 (engine_device_status) and are left out.
  *
  * `slots` (device, n entries; may be null: slot i for entry i) names the slots
  * that a call works on.  k and v are 16-byte aligned.

@@ -390,6 +390,23 @@ def test_bad_entries_are_left_out(pkg, dev):
     assert torch.equal(kv.k, before)
 
 
+@pytest.mark.parametrize("n_tokens", [4095, 16384])
+def test_rows_that_overlap_without_end(pkg, dev, n_tokens):
+    """Row counts that go back and forth, so that 512 sequences have all of the rows: more work
+    than 32 bits count (both attention kernels).  Flagged, nothing done."""
+    hk, group, d, page = 8, 8, 64, 128
+    kv = pkg.ops.PagedKV.empty(1, 2, hk, page, d, 1, 1024, I8, dev)
+    kv.table.zero_()
+    kv.length.fill_(1024 * page)
+    q = torch.zeros(n_tokens, hk * group, d, dtype=torch.float16, device=dev)
+    cu = i32([0, n_tokens] * 512 + [0], dev)
+    out = torch.full_like(q, 3)
+    pkg.ops.attention_paged_prefill(kv, 0, q, torch.zeros(1024, dtype=torch.int32, device=dev), cu, causal=False,
+                                    out=out)
+    assert pkg.device_status() & 2
+    assert out.eq(3).all()
+
+
 def test_codes_past_4_gib(pkg, dev):
     """A pool whose byte offsets pass 32 bits: the last pages."""
     n_pages = 70000  # 8 heads x 64 x 128 bytes each: 4.6 GB a side
