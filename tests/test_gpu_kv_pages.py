@@ -401,7 +401,7 @@ def test_rows_that_overlap_without_end(pkg, dev, n_tokens):
     q = torch.zeros(n_tokens, hk * group, d, dtype=torch.float16, device=dev)
     cu = i32([0, n_tokens] * 512 + [0], dev)
     out = torch.full_like(q, 3)
-    pkg.ops.attention_paged_prefill(kv, 0, q, torch.zeros(1024, dtype=torch.int32, device=dev), cu, causal=False,
+    pkg.ops.attention_paged_prefill(kv, 0, q, torch.zeros(1024, dtype=torch.int32, device=dev), cu, is_causal=False,
                                     out=out)
     assert pkg.device_status() & 2
     assert out.eq(3).all()
