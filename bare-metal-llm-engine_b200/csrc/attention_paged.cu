@@ -30,8 +30,8 @@
 // are consecutive bytes: D / 4 of two keys' rows for S^T, D / 8 of four keys' rows for
 // O^T; P passes from one layout to the other by two 8 x 8 transpositions.
 //   Measured (B200, 32 / 8 heads of 128, calls back to back): 131072 keys of one sequence
-// 55 us (269 MB, 0.75 of the measured copy rate), 48 sequences of 200-16384 keys 72 us (372
-// MB, 0.79), 64 x 4000 keys 94 us (0.85).  Within the kernel the tiles arrive at about 7 TB/s;
+// 54 us (269 MB, 0.75 of the measured copy rate), 48 sequences of 200-16384 keys 74 us (372
+// MB, 0.77), 64 x 4000 keys 94 us (0.85).  Within the kernel the tiles arrive at about 7 TB/s;
 // the rest is the 5 us until the first tile is there (lengths, table, scales and codes, each
 // looked up with the last), the spread of the shares' ends and the join (4 us).  With q as A
 // and the int8 offset taken off every code the first was 66 us where it is 54 to 55.  Eight

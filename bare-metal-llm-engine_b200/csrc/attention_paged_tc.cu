@@ -22,14 +22,14 @@
 // and B.  Within a side, S -> softmax -> P V is a chain; the two sides' chains interleave
 // on the tensor cores and the exponential units.
 //
-//   Measured (B200, 32 / 8 heads of 128, calls back to back): 512 rows on 8704 keys 92 us (771
-// TFLOP/s, 0.46 of the measured burst), a 4096-token prompt 165-180 us.  A side's chain bounds
+//   Measured (B200, 32 / 8 heads of 128, calls back to back): 512 rows on 8704 keys 94 us (753
+// TFLOP/s, 0.45 of the measured burst), a 4096-token prompt 172 us.  A side's chain bounds
 // it: of about 4100 cycles a tile, 700 are the maxima, 1700 the weights (exponentials 512 of
 // each half's 850), 1600 from the last weight to the next tile's S.  Steps: one thread a row
 // with S in 128 registers 117 us; four threads a row 135; one MMA thread for both sides, whose
 // issue was the bound, to a warp a side and descriptors that differ by constants 119; the
-// sides' turns and the maxima before them 93; the first half's scores kept 92.  Without the
-// turns 103.
+// sides' turns and the maxima before them 93; the first half's scores kept 92 to 94.  Without
+// the turns 103.
 //
 // Every wait is bounded (ENGINE_WAIT_TIMEOUT_MS): on expiry the thread sets the device
 // error word, its role ends, the others' waits run out too, and all meet at the
