@@ -58,10 +58,10 @@ constexpr float kPgRescale = 8.0f;
 /// with 2, 72 with 4, 74 with 8.
 constexpr int kPgItemCost = 4;
 /// Query rows of a sequence and KV head (the average: the host knows no more) from which
-/// attention_paged_tc takes the call.  One sequence of 4000 keys: 24 rows 25 us either way, 32
-/// rows 23 us there and 27 here, 64 rows 23 and 29; sixteen of them: 16 rows 83 and 50, 32
-/// rows 80 and 77, 48 rows 82 and 103.
-constexpr int64_t kManyRows = 32;
+/// attention_paged_tc takes the call: what needs a third group of 16 here.  One sequence of
+/// 4000 keys: 32 rows 23 us either way, 48 rows 23 us there and 24 here, 64 rows 23 and 25;
+/// sixteen of them: 16 rows 83 and 52, 32 rows 81 and 77, 48 rows 82 and 103.
+constexpr int64_t kManyRows = 33;
 /// Slots of at most so many tiles have a CTA to an item: no workspace, no join.  1000 keys: one
 /// sequence 13 us and 16 split, 8 sequences 14 and 16, 256 sequences 102 and 103; at 2000 keys
 /// (32 tiles) it would be 21 and 16, 26 and 20, 176 and 179.
@@ -668,9 +668,36 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
   }
 }
 
+/// The k-th (from 0) of the entries that hold a cut item; its x is -1 where there is none.
+/// The whole warp comes with one k.
+__device__ __forceinline__ int4 nth_cut(const int4* cuts, int n, int k) {
+  constexpr int J = 8;
+  for (int base = 0; base < n; base += 32 * J) {
+    int x[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int i = base + 32 * j + static_cast<int>(lane_id());
+      x[j] = i < n ? cuts[i].x : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      unsigned some = __ballot_sync(0xffffffffu, x[j] >= 0);
+      const int count = __popc(some);
+      if (k < count) {
+        for (; k > 0; --k) some &= some - 1;
+        return cuts[base + 32 * j + __ffs(some) - 1];
+      }
+      k -= count;
+    }
+  }
+  return make_int4(-1, 0, 0, 0);
+}
+
 /// Joins the parts of a cut item (part 1 of the CTA that began it, and part 0 of each one
-/// up to that which finished it); blockIdx.x is the entry of p.cut, blockIdx.y the row.  One sequence of 131072 keys has 55 parts of a row: eight warps
-/// take every eighth, so that all of them are on their way at once.
+/// up to that which finished it); blockIdx.x is the item (the entry of p.cut, or, where a
+/// few are spread over many entries, the number among those that hold one), blockIdx.y the
+/// row.  One sequence of 131072 keys has 55 parts of a row: eight warps take every eighth,
+/// so that all of them are on their way at once.
 constexpr int kJoinWarps = 8;
 /// RPB: rows of a block.  One where an item has many parts; eight, a warp each, where it
 /// has a few.
@@ -678,7 +705,7 @@ template <int D, int RPB>
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const ApParams p) {
   pdl_trigger();
   pdl_wait();
-  const int4 cut = p.cut[blockIdx.x];
+  const int4 cut = RPB == 1 && !p.by_item ? nth_cut(p.cut, p.n_cut, blockIdx.x) : p.cut[blockIdx.x];
   if (cut.x < 0) return;
   constexpr int E = D / 32;            // columns of a lane
   constexpr int W = kJoinWarps / RPB;  // warps of a row
@@ -770,6 +797,7 @@ int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most, int64_t 
   // Else they are known by the CTA that began them.
   p.by_item = p.cu == nullptr && items <= ctas ? 1 : 0;
   const int64_t cuts = p.by_item ? items : ctas;
+  p.n_cut = static_cast<int>(cuts);
   const size_t o_bytes = 2 * ctas * kPgRows * D * sizeof(float), ml_bytes = 2 * ctas * kPgRows * sizeof(float2);
   char* ws = static_cast<char*>(scratch_alloc(o_bytes + ml_bytes + cuts * sizeof(int4), st));
   if (ws == nullptr) return set_error(ENGINE_ERR_CUDA, "attention_paged: workspace allocation failed");
@@ -784,8 +812,10 @@ int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most, int64_t 
   cudaError_t e = cudaGetLastError();
   const unsigned c = static_cast<unsigned>(cuts);
   if (e == cudaSuccess) {
+    // With few items a block looks for its entry: of the 444 x 16 that one block an entry and
+    // row would be nearly all had nothing to do (8 rows on 4000 keys 23 us then, 19 so).
     if (ctas >= 8 * items)
-      e = launch_pdl(attn_paged_join_kernel<D, 1>, dim3(c, Cfg::kRows), dim3(kJoinWarps * 32), 0, st, p);
+      e = launch_pdl(attn_paged_join_kernel<D, 1>, dim3(static_cast<unsigned>(items), Cfg::kRows), dim3(kJoinWarps * 32), 0, st, p);
     else
       e = launch_pdl(attn_paged_join_kernel<D, 8>, dim3(c, Cfg::kRows / 8), dim3(kJoinWarps * 32), 0, st, p);
   }

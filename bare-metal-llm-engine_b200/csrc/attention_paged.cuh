@@ -25,6 +25,7 @@ struct ApParams {
   int4* cut;          // items that are cut: sequence (-1: none), first row, KV head (16-row
                       // kernel: and parts << 16), last CTA (16-row kernel: the first)
   int by_item;        // 16-row kernel: cut[item], one row per sequence; else cut[CTA that began it]
+  int n_cut;          // 16-row kernel: entries of cut
   int whole;          // a CTA to an item: none is cut, no workspace
   unsigned long long limit_ns;
 };

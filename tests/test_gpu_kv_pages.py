@@ -316,6 +316,24 @@ def test_pages_of_zeros_beside_small_values(pkg, dev, dtype, new):
     ref.check_attention(kv, 0, q, out, [0], [0, new], d ** -0.5, True, lse)
 
 
+@pytest.mark.parametrize("rows", [[1], [4, 0, 2], [7, 9, 1, 1, 3], [33], [70, 40, 0, 150], [9] * 12])
+def test_prefill_cut_items(pkg, dev, rows):
+    """Rows over a few thousand keys: items cut into many parts, few items or many, both kernels."""
+    n = len(rows)
+    lens = [1400 + 331 * i for i in range(n)]
+    lens[-1] = 40
+    m, kv = make(pkg, dev, hk=2, d=64, page=64, slots=n, n_pages=700, max_pages=100)
+    grow(pkg, m, kv, list(range(n)), lens, dev, 3)
+    cu = [0]
+    for r in rows:
+        cu.append(cu[-1] + r)
+    q = torch.randn(cu[-1], 8, 64, generator=torch.Generator().manual_seed(2)).half().to(dev)
+    out, lse = pkg.ops.attention_paged_prefill(kv, 0, q, None, i32(cu, dev), want_lse=True)
+    ref.check_attention(kv, 0, q, out, list(range(n)), cu, 0.125, True, lse)
+    assert torch.equal(out, pkg.ops.attention_paged_prefill(kv, 0, q, None, i32(cu, dev)))
+    assert pkg.device_status() == 0
+
+
 def test_prefill_rows_that_see_nothing(pkg, dev):
     """More query rows than positions: the first rows see no key."""
     m, kv = make(pkg, dev, hk=2, d=128, page=16)
