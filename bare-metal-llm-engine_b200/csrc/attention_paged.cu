@@ -47,7 +47,7 @@ namespace b200 {
 namespace {
 
 constexpr int kPgKeys = 64;      // keys per tile
-constexpr int kPgRows = 16;      // query rows per item, at most
+constexpr int kPgRows = 16;      // query rows per item, at most (PgCfg::kRows)
 constexpr int kPgConsumers = 4;  // warps; each takes 16 keys of a tile
 constexpr int kPgThreads = (kPgConsumers + 1) * 32;
 constexpr int kPgMaxSeq = 1024;  // sequences per launch (their prefix sums sit in shared memory)
@@ -162,6 +162,7 @@ struct PgLists {
 };
 
 /// The item at step `x` (`whole`: the item of that number), up to step `hi`.
+template <int ROWS>
 __device__ __forceinline__ PgItem pg_item(const ApParams& p, const PgLists& s, int x, int hi) {
   int lo = 0, up = p.n_seq - 1;
   while (lo < up) {  // the last sequence that starts at or before x
@@ -182,7 +183,7 @@ __device__ __forceinline__ PgItem pg_item(const ApParams& p, const PgLists& s, i
   it.t1 = p.whole ? it.tiles : max(min(hi - it.begin - kPgItemCost, it.tiles), it.t0);
   it.end = it.begin + (p.whole ? 1 : kPgItemCost + it.t1);
   it.head = j % p.c.heads;
-  it.row0 = j / p.c.heads * kPgRows;
+  it.row0 = j / p.c.heads * ROWS;
   it.n_tok = kv_rows(p.c, p.cu, p.seq0 + lo, p.n_tokens, &it.first);
   it.n_rows = it.n_tok * p.group;
   return it;
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
     const int rows = kv_rows(p.c, p.cu, p.seq0 + b, p.n_tokens, &first) * p.group;
     s_slot[b] = slot;
     s_len[b] = len;
-    s_pre[b] = (rows + kPgRows - 1) / kPgRows * p.c.heads * (p.whole ? 1 : kPgItemCost + max((len + kPgKeys - 1) / kPgKeys, 1));
+    s_pre[b] = (rows + Cfg::kRows - 1) / Cfg::kRows * p.c.heads * (p.whole ? 1 : kPgItemCost + max((len + kPgKeys - 1) / kPgKeys, 1));
   }
   __syncthreads();
   if (warp == 0) {
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
     int page_base = 0;
     bool ok = true;
     for (int x = lo; x < hi && ok;) {
-      const PgItem it = pg_item(p, lists, x, hi);
+      const PgItem it = pg_item<Cfg::kRows>(p, lists, x, hi);
       x = it.end;
       if (it.t0 == it.t1) break;
       const int n_keys = it.len;
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
     bool ok = true;
     if (threadIdx.x == 0 && !p.whole && !p.by_item) p.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
     for (int x = lo; x < hi;) {
-      const PgItem it = pg_item(p, lists, x, hi);
+      const PgItem it = pg_item<Cfg::kRows>(p, lists, x, hi);
       x = it.end;
       if (it.t0 == it.t1) break;
       // q^T as B fragments: the lane's D / 4 elements of query row g (and g + 8), from
@@ -659,7 +660,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
       }
       if (threadIdx.x == 0 && it.t0 == 0 && !p.whole && (p.by_item || !whole)) {
         const int parts = (it.begin + kPgItemCost + it.tiles - 1) / per - static_cast<int>(blockIdx.x) + 1;
-        const int at = p.by_item ? (it.b * ((p.group + kPgRows - 1) / kPgRows) + it.row0 / kPgRows) * p.c.heads + it.head
+        const int at = p.by_item ? (it.b * ((p.group + Cfg::kRows - 1) / Cfg::kRows) + it.row0 / Cfg::kRows) * p.c.heads + it.head
                                  : static_cast<int>(blockIdx.x);
         p.cut[at] = make_int4(whole ? -1 : it.b, it.row0, it.head | parts << 16, static_cast<int>(blockIdx.x));
       }
@@ -813,7 +814,7 @@ int launch_paged(ApParams p, const engine_kv_pages_t* kv, int64_t most, int64_t 
   const unsigned c = static_cast<unsigned>(cuts);
   if (e == cudaSuccess) {
     // With few items a block looks for its entry: of the 444 x 16 that one block an entry and
-    // row would be nearly all had nothing to do (8 rows on 4000 keys 23 us then, 19 so).
+    // row would be nearly all had nothing to do (16 rows on 4000 keys 25 us then, 21 so).
     if (ctas >= 8 * items)
       e = launch_pdl(attn_paged_join_kernel<D, 1>, dim3(static_cast<unsigned>(items), Cfg::kRows), dim3(kJoinWarps * 32), 0, st, p);
     else
@@ -829,9 +830,13 @@ int run_paged(ApParams p, const engine_kv_pages_t* kv, int64_t n_seq, cudaStream
   const bool e4m3 = kv->type == ENGINE_KV_E4M3;
   const int64_t tiles = std::max<int64_t>((kv->max_pages * kv->page_size + kPgKeys - 1) / kPgKeys, 1);
   const int64_t steps = tiles + kPgItemCost;
-  const bool r8 = p.cu == nullptr && p.group <= 8;
-  // Rows per sequence and KV head, on the average (the host knows no more).
-  const bool many = p.cu != nullptr && p.group <= 128 && p.n_tokens * p.group >= kManyRows * n_seq;
+  // Rows per sequence and KV head, on the average (the host knows no more).  Where that is at
+  // most 8 an item has 8 rows (8 of 16 sequences of 4000 keys 37 us, 50 with items of 16; of
+  // one sequence 16 and 19), else 16, so that the keys are read half as often.
+  const int64_t all = p.cu == nullptr ? p.group * n_seq : p.n_tokens * p.group;
+  const bool r8 = all <= 8 * n_seq;
+  const bool many = p.cu != nullptr && p.group <= 128 && all >= kManyRows * n_seq;
+  const int64_t rows = r8 ? 8 : 16;  // of an item
   for (int64_t at = 0; at < n_seq; at += kPgMaxSeq) {
     const int64_t n = std::min<int64_t>(kPgMaxSeq, n_seq - at);
     p.seq0 = static_cast<int>(at);
@@ -841,8 +846,8 @@ int run_paged(ApParams p, const engine_kv_pages_t* kv, int64_t n_seq, cudaStream
       continue;
     }
     // At most this many steps (the kernel counts them in 32 bits).
-    const int64_t groups = p.cu == nullptr ? n * ((p.group + kPgRows - 1) / kPgRows)
-                                           : p.n_tokens * p.group / kPgRows + n;
+    const int64_t groups = p.cu == nullptr ? n * ((p.group + rows - 1) / rows)
+                                           : p.n_tokens * p.group / rows + n;
     if (groups > 0x7fffffff / kv->n_kv_heads / steps)
       return set_error(ENGINE_ERR_UNSUPPORTED, std::string(what) + ": too many query rows x positions");
     p.whole = tiles <= kWholeTiles ? 1 : 0;
