@@ -202,8 +202,10 @@ struct TcBars {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];  // stages
   uint64_t s_full[2], p_full[2][2];                       // sides, halves of 64 keys
   uint64_t o_done[2], o_free[2], drain[2];                // sides
+  uint64_t b_turn;                                        // tiles that side B is done with
   uint32_t tmem;
 };
+static_assert(sizeof(TcBars) <= 256, "space of the barriers");
 
 /// A softmax warp has 16 rows of a side; a thread two of them (lane / 4 and + 8) and, of
 /// every 8 columns, 2 (lane % 4) and the next: 32 values of a half tile of 64 keys, in
@@ -319,6 +321,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (threadIdx.x == 0) {
     mbar_init(&bar->q_full, 1);
     mbar_init(&bar->q_empty, 2);
+    mbar_init(&bar->b_turn, 8);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bar->raw_full[s], 1);
       mbar_init(&bar->raw_empty[s], 4);
@@ -460,7 +463,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int g = lane >> 2, t4 = lane & 3;
     const uint32_t tS = tmem + (static_cast<uint32_t>(r0) << 16) + side * 128;
     const uint32_t tO = tmem + (static_cast<uint32_t>(r0) << 16) + Cfg::kColO + side * D;
-    int n = 0, nb = 0;  // tiles, and those that B had a part in
+    int n = 0, own = 0;  // tiles, and those of this side
     bool ok = true;
     // Token within the side's, or far past any, and head within the group of the thread's rows.
     int q_tok[2], q_head[2];
@@ -472,7 +475,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int x = lo; x < hi && ok && it.t0 < it.t1;) {
       if (side == 1 && !it.two) {
-        n += it.t1 - it.t0;
+        // No rows: A's turns are followed all the same (see below).
+        for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
+          ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->p_full[0][1], n & 1, limit, c.err));
+          if (ok && lane == 0) mbar_arrive(&bar->b_turn);
+          __syncwarp();
+        }
         x = tc_end(it);
         if (x < hi) tc_next(p, it, x, hi);
         continue;
@@ -483,10 +491,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int r = 0; r < 2; ++r)
         lim[r] = p.a.causal && q_tok[r] < left ? it.len - left + q_tok[r] + 1 : it.len;
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-      for (int t = it.t0; t < it.t1; ++t, ++n, nb += it.two ? 1 : 0) {
+      for (int t = it.t0; t < it.t1; ++t, ++n, ++own) {
         const float4* con = s_const + (n & 3) * 8;
         const int key = t * kTcKeys + 2 * t4;
-        ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->s_full[side], (side ? nb : n) & 1, limit, c.err));
+        ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->s_full[side], own & 1, limit, c.err));
         if (!ok) break;
         tc_fence_after();
         const bool clean =
@@ -527,12 +535,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
         }
-        // The sides' exponentials take turns: A after B's last tile, B after A's this one.  In
-        // step, both would want them at once and both would then want the tensor cores.
-        // (A waits in items without a side B too, so that it is never two tiles ahead of B's wait.)
-        if (side == 1 || nb > 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->p_full[side ^ 1][1], side ? n & 1 : (nb - 1) & 1,
-                                                        limit, c.err));
+        // The sides' exponentials take turns, tile by tile: A after B's last one, B after A's this
+        // one.  In step, both would want them at once and both would then want the tensor cores.
+        // B takes its turn, empty-handed, in the tiles of items without a side B too: a wait tells
+        // apart two phases only, so neither side may be two tiles ahead of the other's wait.
+        if (side == 1 || n > 0) {
+          ok = __all_sync(0xffffffffu, side ? mbar_wait_sleepy(&bar->p_full[0][1], n & 1, limit, c.err)
+                                            : mbar_wait_sleepy(&bar->b_turn, (n - 1) & 1, limit, c.err));
           if (!ok) break;
         }
 #pragma unroll
@@ -546,6 +555,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tc_fence_before();
           mbar_arrive(&bar->p_full[side][half]);
         }
+        if (side == 1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar->b_turn);
+        }
       }
       if (!ok) break;
 #pragma unroll
@@ -553,7 +566,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
       }
-      ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->o_done[side], ((side ? nb : n) - 1) & 1, limit, c.err));
+      ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->o_done[side], (own - 1) & 1, limit, c.err));
       if (!ok) break;
       tc_fence_after();
       const bool whole = it.t1 - it.t0 == it.tiles;

@@ -334,6 +334,32 @@ def test_prefill_cut_items(pkg, dev, rows):
     assert pkg.device_status() == 0
 
 
+@pytest.mark.parametrize("heads,hk,d", [(192, 3, 64), (32, 2, 64), (32, 8, 128)])
+def test_prefill_items_without_a_second_side(pkg, dev, heads, hk, d):
+    """Short sequences with odd tails, so that items of one tile with and without rows in the
+    second half follow each other: every call answers the same, no wait runs out."""
+    rnd = random.Random(4)
+    n = 17
+    lens = [rnd.choice([0, 1, 3, rnd.randint(1, 200), 128, 130]) for _ in range(n)]
+    rows = [rnd.choice([1, 33, 65, rnd.randint(30, 300), 128]) for _ in range(n)]
+    m, kv = make(pkg, dev, hk=hk, d=d, page=32, slots=n, n_pages=120, max_pages=9, dtype=E4M3)
+    grow(pkg, m, kv, list(range(n)), lens, dev, 3)
+    cu = [0]
+    for r in rows:
+        cu.append(cu[-1] + r)
+    q = torch.randn(cu[-1], heads, d, generator=torch.Generator().manual_seed(2)).half().to(dev)
+    first = None
+    for _ in range(25):
+        out = torch.full_like(q, 7)
+        pkg.ops.attention_paged_prefill(kv, 0, q, None, i32(cu, dev), out=out)
+        first = out if first is None else first
+        assert torch.equal(out, first)
+    assert pkg.device_status() == 0
+    for b in (2, 7, 11, 16):  # the last rows of some
+        at = slice(cu[b + 1] - min(rows[b], 3), cu[b + 1])
+        ref.check_attention(kv, 0, q[at], first[at], [b], [0, min(rows[b], 3)], d ** -0.5)
+
+
 def test_prefill_rows_that_see_nothing(pkg, dev):
     """More query rows than positions: the first rows see no key."""
     m, kv = make(pkg, dev, hk=2, d=128, page=16)
