@@ -202,7 +202,7 @@ struct TcBars {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];  // stages
   uint64_t s_full[2], p_full[2][2];                       // sides, halves of 64 keys
   uint64_t o_done[2], o_free[2], drain[2];                // sides
-  uint64_t b_turn;                                        // tiles that side B is done with
+  uint64_t a_turn;                                        // A's weights, in items with a side B
   uint32_t tmem;
 };
 static_assert(sizeof(TcBars) <= 256, "space of the barriers");
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (threadIdx.x == 0) {
     mbar_init(&bar->q_full, 1);
     mbar_init(&bar->q_empty, 2);
-    mbar_init(&bar->b_turn, 8);
+    mbar_init(&bar->a_turn, 8);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bar->raw_full[s], 1);
       mbar_init(&bar->raw_empty[s], 4);
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int g = lane >> 2, t4 = lane & 3;
     const uint32_t tS = tmem + (static_cast<uint32_t>(r0) << 16) + side * 128;
     const uint32_t tO = tmem + (static_cast<uint32_t>(r0) << 16) + Cfg::kColO + side * D;
-    int n = 0, own = 0;  // tiles, and those of this side
+    int n = 0, own = 0, both = 0;  // tiles, those of this side, and those with a side B
     bool ok = true;
     // Token within the side's, or far past any, and head within the group of the thread's rows.
     int q_tok[2], q_head[2];
@@ -475,12 +475,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int x = lo; x < hi && ok && it.t0 < it.t1;) {
       if (side == 1 && !it.two) {
-        // No rows: A's turns are followed all the same (see below).
-        for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
-          ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->p_full[0][1], n & 1, limit, c.err));
-          if (ok && lane == 0) mbar_arrive(&bar->b_turn);
-          __syncwarp();
-        }
+        n += it.t1 - it.t0;
         x = tc_end(it);
         if (x < hi) tc_next(p, it, x, hi);
         continue;
@@ -491,7 +486,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int r = 0; r < 2; ++r)
         lim[r] = p.a.causal && q_tok[r] < left ? it.len - left + q_tok[r] + 1 : it.len;
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-      for (int t = it.t0; t < it.t1; ++t, ++n, ++own) {
+      for (int t = it.t0; t < it.t1; ++t, ++n, ++own, both += it.two ? 1 : 0) {
         const float4* con = s_const + (n & 3) * 8;
         const int key = t * kTcKeys + 2 * t4;
         ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->s_full[side], own & 1, limit, c.err));
@@ -535,13 +530,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
         }
-        // The sides' exponentials take turns, tile by tile: A after B's last one, B after A's this
-        // one.  In step, both would want them at once and both would then want the tensor cores.
-        // B takes its turn, empty-handed, in the tiles of items without a side B too: a wait tells
-        // apart two phases only, so neither side may be two tiles ahead of the other's wait.
-        if (side == 1 || n > 0) {
-          ok = __all_sync(0xffffffffu, side ? mbar_wait_sleepy(&bar->p_full[0][1], n & 1, limit, c.err)
-                                            : mbar_wait_sleepy(&bar->b_turn, (n - 1) & 1, limit, c.err));
+        // The sides' exponentials take turns: A after B's last tile, B after A's this one.  In
+        // step, both would want them at once and both would then want the tensor cores.  Both
+        // count the tiles of items with a side B alone (a wait tells apart two phases only, and
+        // A may be any number of other tiles ahead).
+        if (side == 1 || (it.two && both > 0)) {
+          ok = __all_sync(0xffffffffu, side ? mbar_wait_sleepy(&bar->a_turn, both & 1, limit, c.err)
+                                            : mbar_wait_sleepy(&bar->p_full[1][1], (both - 1) & 1, limit, c.err));
           if (!ok) break;
         }
 #pragma unroll
@@ -555,9 +550,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tc_fence_before();
           mbar_arrive(&bar->p_full[side][half]);
         }
-        if (side == 1) {
+        if (side == 0 && it.two) {
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bar->b_turn);
+          if (lane == 0) mbar_arrive(&bar->a_turn);
         }
       }
       if (!ok) break;
