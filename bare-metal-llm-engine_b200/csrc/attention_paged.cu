@@ -320,7 +320,10 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
         // At the CTA's start the first tiles are on their way before the scales are here.
         int ahead = 0;
         if (n == 0) {
-          for (; ahead < min(count, ST) && ok; ++ahead) fetch(ahead, ahead);
+          while (ahead < min(count, ST) && ok) {
+            fetch(ahead, ahead);
+            if (ok) ++ahead;
+          }
         }
         const float v1 = vs == 0.0f ? kNoScale : vs;
         const float4 con = id >= 0 ? make_float4(ks * kc_unit, log2f(v1), 1.0f / v1, 1.0f)
@@ -357,7 +360,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
         __syncwarp();
       }
     }
-    for (int j = max(n - ST, 0); j < n; ++j) mbar_wait(&full[j % ST], (j / ST) & 1u, p.limit_ns, p.c.err);
+    for (int j = max(n - ST, 0); j < n; ++j) mbar_wait(&full[j % ST], (j / ST) & 1u, drain_ns(p.limit_ns), p.c.err);
   } else {
     // ----------------------------------------------------------- consumers
     const int g = lane >> 2, t = lane & 3;

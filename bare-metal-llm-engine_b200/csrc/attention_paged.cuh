@@ -35,6 +35,12 @@ struct ApParams {
 constexpr int kTcMaxSeq = 1024;
 int attention_paged_tc(const ApParams& p, const engine_kv_pages_t* kv, cudaStream_t st);
 
+/// The limit of a wait for a CTA's own copies and products in flight.  They end by themselves, and
+/// the CTA must not leave before them, however short the limit of its roles' waits for each other is.
+__device__ __forceinline__ unsigned long long drain_ns(unsigned long long limit_ns) {
+  return limit_ns > 2000000000ull ? limit_ns : 2000000000ull;
+}
+
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

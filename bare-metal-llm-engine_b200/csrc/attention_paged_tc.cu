@@ -31,9 +31,9 @@
 // sides' turns and the maxima before them 93; the first half's scores kept 92 to 94.  Without
 // the turns 103 (four prompts of 700-5000 tokens 406, 378 with them).
 //
-// Every wait is bounded (ENGINE_WAIT_TIMEOUT_MS): on expiry the thread sets the device
+// Every wait is bounded (ENGINE_WAIT_TIMEOUT_MS): on expiry the warp sets the device
 // error word, its role ends, the others' waits run out too, and all meet at the
-// teardown, where copies and MMAs in flight are waited for.
+// teardown, where copies and MMAs in flight are waited for (by a limit of their own).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -615,11 +615,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       x = tc_end(it);
       if (x < hi) tc_next(p, it, x, hi);
     }
+    __syncwarp();
+    tmem_wait_st();  // behind a wait that ran out, a rescaled O may still be on its way
   } else {
     set_max_regs_dec<kRegsOther>();
     if (warp == 20) {
       // ----------------------------------------------------- lookups and TMA
-      int n = 0, items = 0;
+      int n = 0, items = 0;  // tiles and items whose copies are on their way
+      int n_k = 0;           // tiles whose K is
       bool ok = true;
       int4 cut = make_int4(-1, 0, 0, 0);
       const int per_box = min(4, 1 << (c.shift - 4));  // slices of 16 keys in a TMA box
@@ -670,6 +673,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               __syncwarp();
               if (lane == 0) mbar_arrive_expect_tx(&bar->raw_full[kv], __popc(who) * per_box * 16 * D);
               __syncwarp();
+              n_k += kv == 0 ? 1 : 0;
               if (mine)
                 tma_load_2d(smem + Cfg::kOffRaw + kv * Cfg::kRaw + slice * 16 * D, kv ? &tmV : &tmK,
                             &bar->raw_full[kv], 0, D == 128 ? row : row >> 1);
@@ -683,11 +687,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (lane == 0) p.a.cut[blockIdx.x] = cut;
       // No copy may still be writing shared memory when the CTA leaves: what was issued last.
-      if (items > 0) mbar_wait(&bar->q_full, (items - 1) & 1, limit, c.err);
-      if (n > 0) {
-        mbar_wait(&bar->raw_full[0], (n - 1) & 1, limit, c.err);
-        mbar_wait(&bar->raw_full[1], (n - 1) & 1, limit, c.err);
-      }
+      // (Behind a wait that ran out that may be a tile's K without its V.)
+      const unsigned long long drain = drain_ns(limit);
+      if (items > 0) mbar_wait(&bar->q_full, (items - 1) & 1, drain, c.err);
+      if (n_k > 0) mbar_wait(&bar->raw_full[0], (n_k - 1) & 1, drain, c.err);
+      if (n > 0) mbar_wait(&bar->raw_full[1], (n - 1) & 1, drain, c.err);
       __syncwarp();
     } else if (warp == 21 || warp == 22) {
       // ----------------------------------------------- MMA, a warp per side
@@ -706,15 +710,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       int items = 0, own = 0;  // items, and this side's
       bool ok = true;
       bool busy = false;  // something was issued
+      // The warp goes on as one: a lane whose wait alone ran out would miss the others' votes.
+      auto wait = [&](uint64_t* b, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(b, parity, limit, c.err));
+      };
       auto pv = [&](int i, bool start) {  // O += P V of tile i, this side's last one; `start`: the item's first
-        ok = mbar_wait(&bar->v_full[i & 1], (i >> 1) & 1, limit, c.err);
+        ok = wait(&bar->v_full[i & 1], (i >> 1) & 1);
         // It overwrites O: the last item's rows have been read.
-        if (ok && start) ok = mbar_wait(&bar->o_free[side], (own & 1) ^ 1u, limit, c.err);
+        if (ok && start) ok = wait(&bar->o_free[side], (own & 1) ^ 1u);
         const uint64_t d = dv + static_cast<uint64_t>((i & 1) * (Cfg::kWide >> 4));
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          if (ok) ok = mbar_wait(&bar->p_full[side][half], (mine - 1) & 1, limit, c.err);
-          ok = __all_sync(0xffffffffu, ok);
+          if (ok) ok = wait(&bar->p_full[side][half], (mine - 1) & 1);
           if (!ok) return;
           tc_fence_after();
           if (leader) {
@@ -732,13 +739,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       };
       for (int x = lo; x < hi && ok && it.t0 < it.t1; ++items) {
-        ok = mbar_wait(&bar->q_full, items & 1, limit, c.err);
+        ok = wait(&bar->q_full, items & 1);
         if (side == 1 && !it.two) {
           // No rows here: the tiles are only given back.
           for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
-            ok = mbar_wait(&bar->k_full[n & 1], (n >> 1) & 1, limit, c.err);
-            if (ok) ok = mbar_wait(&bar->v_full[n & 1], (n >> 1) & 1, limit, c.err);
-            ok = __all_sync(0xffffffffu, ok);
+            ok = wait(&bar->k_full[n & 1], (n >> 1) & 1);
+            if (ok) ok = wait(&bar->v_full[n & 1], (n >> 1) & 1);
             if (ok && leader) {
               mbar_arrive(&bar->k_empty[n & 1]);
               mbar_arrive(&bar->v_empty[n & 1]);
@@ -749,11 +755,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           __syncwarp();
         } else {
           for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
-            ok = mbar_wait(&bar->k_full[n & 1], (n >> 1) & 1, limit, c.err);
+            ok = wait(&bar->k_full[n & 1], (n >> 1) & 1);
             if (ok && t > it.t0) pv(n - 1, t == it.t0 + 1);
             // S goes over P of the tile before: its product must have read it.
-            if (ok && mine > 0) ok = mbar_wait(&bar->o_done[side], (mine - 1) & 1, limit, c.err);
-            ok = __all_sync(0xffffffffu, ok);
+            if (ok && mine > 0) ok = wait(&bar->o_done[side], (mine - 1) & 1);
             if (!ok) break;
             tc_fence_after();
             if (leader) {
@@ -782,7 +787,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (busy) {
         if (leader) umma_commit(&bar->drain[side]);
         __syncwarp();
-        mbar_wait(&bar->drain[side], 0, limit, c.err);
+        mbar_wait(&bar->drain[side], 0, drain_ns(limit), c.err);
       }
     }
     __syncwarp();

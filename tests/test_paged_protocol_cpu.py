@@ -1,0 +1,44 @@
+"""CPU: the order of the tcgen05 paged attention kernel's roles (tests/paged_protocol.py)."""
+from __future__ import annotations
+
+import random
+
+import pytest
+
+from tests.paged_protocol import Cta, random_items
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_roles_go_through_in_any_order(seed):
+    """Every row of every item is stored, whatever the order of events."""
+    rng = random.Random(seed)
+    for _ in range(60):
+        items = random_items(rng)
+        cta = Cta(items, rng)
+        assert not cta.run()
+        assert cta.stored == {(i, s): t for i, (t, two) in enumerate(items) for s in range(1 + two)}
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_waits_that_run_out_leave_nothing_in_flight(seed):
+    """Waits that give up anywhere: all roles end, copies and products have landed, and what is
+    stored is complete."""
+    rng = random.Random(100 + seed)
+    gave_up = 0
+    for _ in range(120):
+        gave_up += Cta(random_items(rng), rng, give_up=rng.choice([0.002, 0.01, 0.05])).run()
+    assert gave_up > 30
+
+
+def test_a_copy_that_is_not_counted_is_found():
+    """A producer that forgets a tile's K where the wait for V's place gave up."""
+    rng = random.Random(7)
+    found = 0
+    for _ in range(400):
+        try:
+            Cta(random_items(rng), rng, give_up=0.02, forget_k=True).run()
+        except AssertionError as e:
+            # left early, or waiting for a phase that the forgotten copy has passed
+            assert "in flight" in str(e) or "two phases apart" in str(e)
+            found += 1
+    assert found > 0
