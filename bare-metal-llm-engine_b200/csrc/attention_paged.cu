@@ -82,7 +82,8 @@ struct PgCfg {
   static constexpr int kOffQ = kOffO + kBufs * kRows * kOW * 4;  // [D / 16][32 lanes], 16 bytes each
   static constexpr int kOffConst = kOffQ + (NQ == 1 ? 0 : D / 16 * 512);
   static constexpr int kOffBar = kOffConst + kStages * 4 * 16;
-  static constexpr int kOffMl = kOffBar + 2 * kStages * 8;
+  static constexpr int kOffFail = kOffBar + 2 * kStages * 8;
+  static constexpr int kOffMl = kOffFail + 16;
   static constexpr int kOffSeq = kOffMl + kPgConsumers * kRows * 8;
   static size_t smem(int n_seq) { return kOffSeq + 12 * (static_cast<size_t>(n_seq) + 1) + 1024; }
 };
@@ -209,6 +210,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
   float4* s_const = reinterpret_cast<float4*>(smem + Cfg::kOffConst);  // [ST][4]: of 16 keys each
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
   uint64_t* empty = full + ST;
+  volatile int* s_fail = reinterpret_cast<int*>(smem + Cfg::kOffFail);  // a consumer's wait ran out
   float2* s_ml = reinterpret_cast<float2*>(smem + Cfg::kOffMl);        // [warps][rows]
   int32_t* s_pre = reinterpret_cast<int32_t*>(smem + Cfg::kOffSeq);    // [n_seq + 1]
   int32_t* s_slot = s_pre + p.n_seq + 1;
@@ -220,6 +222,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], kPgConsumers);
     }
+    *s_fail = 0;
     fence_barrier_init();
     prefetch_tmap(&tmK);
     prefetch_tmap(&tmV);
@@ -592,6 +595,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
           if (g == 0) s_ml[warp * Cfg::kRows + 8 * nq + 2 * t + e] = make_float2(m[nq][e], l[nq][e]);
         }
       }
+      if (!ok) *s_fail = 1;  // rows without this warp's keys: none go out from here on
       consumer_sync();
       float a[NQ][2];
 #pragma unroll
@@ -648,8 +652,9 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
           const float4 y = *reinterpret_cast<const float4*>(s_o + (w * Cfg::kRows + row) * Cfg::kOW + col);
           u = make_float4(u.x + y.x, u.y + y.y, u.z + y.z, u.w + y.w);
         }
+        const bool complete = *s_fail == 0;
         if (whole) {
-          if (!ok) continue;
+          if (!complete) continue;
           const int64_t at = pg_row(p, it.first, it.head, it.row0 + row);
           const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
           const __half2 h[2] = {__floats2half2_rn(u.x * inv, u.y * inv), __floats2half2_rn(u.z * inv, u.w * inv)};
@@ -658,7 +663,7 @@ __global__ void __launch_bounds__(kPgThreads, PgCfg<D, NQ>::kCtas)
             p.lse[at] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
         } else {
           *reinterpret_cast<float4*>(p.ws_o + (static_cast<int64_t>(wslot) * kPgRows + row) * D + col) = u;
-          if (col == 0) p.ws_ml[wslot * kPgRows + row] = make_float2(mm, ll);
+          if (col == 0) p.ws_ml[wslot * kPgRows + row] = make_float2(mm, complete ? ll : kNoPart);
         }
       }
       if (threadIdx.x == 0 && it.t0 == 0 && !p.whole && (p.by_item || !whole)) {
@@ -724,7 +729,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
   const int part0 = 2 * cut.w;
   auto slot = [&](int i) { return static_cast<int64_t>(part0 + (i == 0 ? 1 : 2 * i)) * kPgRows + row; };
   float m = -INFINITY;
-  for (int i = lane; i < parts; i += 32) m = fmaxf(m, p.ws_ml[slot(i)].x);
+  bool all = true;
+  for (int i = lane; i < parts; i += 32) {
+    const float2 ml = p.ws_ml[slot(i)];
+    m = fmaxf(m, ml.x);
+    all &= ml.y != kNoPart;
+  }
+  if (!__all_sync(0xffffffffu, all)) return;  // (every warp of a row looks at all parts)
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
   float l = 0.0f, o[E] = {};

@@ -35,6 +35,10 @@ struct ApParams {
 constexpr int kTcMaxSeq = 1024;
 int attention_paged_tc(const ApParams& p, const engine_kv_pages_t* kv, cudaStream_t st);
 
+/// l of a part that was not stored (a wait ran out), which no sum of weights is: the join then
+/// leaves the row as it was, as the kernels leave the rows of items that are not cut.
+constexpr float kNoPart = -1.0f;
+
 /// The limit of a wait for a CTA's own copies and products in flight.  They end by themselves, and
 /// the CTA must not leave before them, however short the limit of its roles' waits for each other is.
 __device__ __forceinline__ unsigned long long drain_ns(unsigned long long limit_ns) {

@@ -347,6 +347,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
   pdl_trigger();
   pdl_wait();
+  // Its two parts are not stored yet.
+  if (threadIdx.x < 2 * kTcRows) p.a.ws_ml[blockIdx.x * (2 * kTcRows) + threadIdx.x] = make_float2(-INFINITY, kNoPart);
+  static_assert(2 * kTcRows <= kTcThreads, "a mark a thread");
   // Steps of each sequence (a warp each), then their sums.  A CTA's share can end within an
   // item's leading steps: it then has no tile of it (t0 == t1), and nothing behind it either.
   for (int b = warp; b < p.a.n_seq; b += kTcThreads / 32) {
@@ -819,8 +822,14 @@ __global__ void __launch_bounds__(2 * D) attn_paged_tc_join_kernel(const TcParam
     return (static_cast<int64_t>(blockIdx.x) * 2 + (i == 0 ? 1 : 2 * i)) * kTcRows + flat;
   };
   float m = -INFINITY;
+  bool all = true;
 #pragma unroll 4
-  for (int i = 0; i < parts; ++i) m = fmaxf(m, p.a.ws_ml[part(i)].x);
+  for (int i = 0; i < parts; ++i) {
+    const float2 ml = p.a.ws_ml[part(i)];
+    m = fmaxf(m, ml.x);
+    all &= ml.y != kNoPart;
+  }
+  if (!all) return;
   float l = 0.0f;
   float4 o = make_float4(0, 0, 0, 0);
 #pragma unroll 2

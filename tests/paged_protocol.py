@@ -1,6 +1,8 @@
-"""The roles of attn_paged_tc_kernel (csrc/attention_paged_tc.cu) and their barriers, restated on
-the host: one CTA's producer, widening warps, softmax and MMA warps of both sides as generators,
-copies and matrix products as agents that end at any later time, and any wait may give up.
+"""The roles of the paged attention kernels and their barriers, restated on the host: of one CTA
+of attn_paged_tc_kernel (csrc/attention_paged_tc.cu) the producer, the widening warps, the softmax
+and MMA warps of both sides; of one of attn_paged_kernel (csrc/attention_paged.cu) the producer
+and the four consumer warps.  Roles are generators, copies and matrix products agents that end at
+any later time, and any wait may give up.
 
 A run checks what the kernel's order rests on: no wait tells two phases apart wrongly, every read
 finds the tile that it is meant to, rows go out only when their products are complete, every role
@@ -35,24 +37,14 @@ class Barrier:
         return (self.done & 1) != (k & 1)
 
 
-class Cta:
-    """items: [(tiles, side B has rows)] of one CTA, in order."""
+class Run:
+    """What the two kernels' CTAs have in common."""
 
-    def __init__(self, items, rng, give_up=0.0, forget_k=False):
-        self.items, self.rng, self.give_up, self.forget_k = items, rng, give_up, forget_k
-        b = Barrier
-        self.q_full, self.q_empty, self.a_turn = b(1), b(2), b(1)
-        self.raw_full, self.raw_empty = [b(1), b(1)], [b(1), b(1)]
-        self.full = [[b(1), b(1)], [b(1), b(1)]]    # K, V; stages
-        self.empty = [[b(2), b(2)], [b(2), b(2)]]
-        self.s_full, self.o_done, self.o_free, self.drain = ([b(1), b(1)] for _ in range(4))
-        self.p_full = [[b(1), b(1)], [b(1), b(1)]]  # sides, halves
+    def __init__(self, items, rng, give_up):
+        self.items, self.rng, self.give_up = items, rng, give_up
         self.copies = []          # (barrier, where, what)
-        self.queue = [[], []]     # of each side's MMA warp, in order
         self.mem = {}             # what is where
-        self.stored = {}          # (item, side) -> tiles in O
-
-    # ---- agents
+        self.stored = {}
 
     def copy(self, bar, where, what):
         self.mem[where] = None
@@ -60,14 +52,71 @@ class Cta:
         self.copies.append((bar, where, what))
 
     def agents(self):
-        ready = [("copy", i) for i in range(len(self.copies))]
-        return ready + [("mma", s) for s in (0, 1) if self.queue[s]]
+        return [("copy", i) for i in range(len(self.copies))]
+
+    def agent(self, kind, i):
+        bar, where, what = self.copies.pop(i)
+        self.mem[where] = what
+        bar.complete()
+
+    def run(self):
+        """Whether a wait gave up.  Roles and agents go on in a random order."""
+        roles = dict.fromkeys(self.roles())
+        for r in list(roles):
+            self._resume(roles, r, None)
+        gave_up = False
+        while roles:
+            ready = [r for r, w in roles.items() if w is None or w[0].passed(w[1])]
+            moves = [("role", r) for r in ready] + self.agents()
+            late = [r for r, w in roles.items() if w is not None and len(w) == 2]
+            if late and (not moves or self.rng.random() < self.give_up):
+                assert self.give_up > 0, "every role waits for another"
+                gave_up = True
+                self._resume(roles, self.rng.choice(late), False)
+            else:
+                assert moves, "a wait for copies or products that were never issued"
+                kind, *what = self.rng.choice(moves)
+                if kind == "role":
+                    self._resume(roles, what[0], True)
+                else:
+                    self.agent(kind, what[0])
+        assert not self.agents(), "something is in flight behind the last role"
+        return gave_up
+
+    def _resume(self, roles, r, answer):
+        try:
+            roles[r] = r.send(answer)
+        except StopIteration:
+            del roles[r]
+
+
+class Cta(Run):
+    """items: [(tiles, side B has rows)] of one CTA, in order."""
+
+    def __init__(self, items, rng, give_up=0.0, forget_k=False):
+        super().__init__(items, rng, give_up)
+        self.forget_k = forget_k
+        b = Barrier
+        self.q_full, self.q_empty, self.a_turn = b(1), b(2), b(1)
+        self.raw_full, self.raw_empty = [b(1), b(1)], [b(1), b(1)]
+        self.full = [[b(1), b(1)], [b(1), b(1)]]    # K, V; stages
+        self.empty = [[b(2), b(2)], [b(2), b(2)]]
+        self.s_full, self.o_done, self.o_free, self.drain = ([b(1), b(1)] for _ in range(4))
+        self.p_full = [[b(1), b(1)], [b(1), b(1)]]  # sides, halves
+        self.queue = [[], []]     # of each side's MMA warp, in order
+        # stored: (item, side) -> tiles in O
+
+    def roles(self):
+        return self.producer(), self.widen(), self.softmax(0), self.softmax(1), self.mma(0), self.mma(1)
+
+    # ---- agents
+
+    def agents(self):
+        return super().agents() + [("mma", s) for s in (0, 1) if self.queue[s]]
 
     def agent(self, kind, i):
         if kind == "copy":
-            bar, where, what = self.copies.pop(i)
-            self.mem[where] = what
-            bar.complete()
+            super().agent(kind, i)
             return
         op = self.queue[i].pop(0)
         if op[0] == "commit":
@@ -218,37 +267,96 @@ class Cta:
             put(("commit", self.drain[side]))
             yield self.drain[side], 0, "drain"
 
-    # ---- a run
 
-    def run(self):
-        """Whether a wait gave up.  Roles and agents go on in a random order."""
-        roles = {r: None for r in (self.producer(), self.widen(), self.softmax(0), self.softmax(1), self.mma(0), self.mma(1))}
-        for r in list(roles):
-            self._resume(roles, r, None)
-        gave_up = False
-        while roles:
-            ready = [r for r, w in roles.items() if w is None or w[0].passed(w[1])]
-            moves = [("role", r) for r in ready] + self.agents()
-            late = [r for r, w in roles.items() if w is not None and len(w) == 2]
-            if late and (not moves or self.rng.random() < self.give_up):
-                assert self.give_up > 0, "every role waits for another"
-                gave_up = True
-                self._resume(roles, self.rng.choice(late), False)
+class FewRows(Run):
+    """items: tiles of each.  forget: a warp whose wait ran out keeps its own rows back only."""
+
+    STAGES, WARPS = 3, 4
+
+    def __init__(self, items, rng, give_up=0.0, forget=False):
+        super().__init__([t for t in items], rng, give_up)
+        self.forget = forget
+        self.full = [Barrier(1) for _ in range(self.STAGES)]
+        self.empty = [Barrier(self.WARPS) for _ in range(self.STAGES)]
+        self.meet = Barrier(self.WARPS)
+        self.fail = False
+        self.seen = {}            # item -> (warp, tile) that its sums hold
+        self.kept = set()         # items whose rows were left as they were, or marked
+
+    def roles(self):
+        return [self.producer()] + [self.consumer(w) for w in range(self.WARPS)]
+
+    def producer(self):
+        n = issued = 0
+        ok, st = True, self.STAGES
+        for tiles in self.items:
+            for base in range(0, tiles, 8):
+                count, ahead = min(8, tiles - base), 0
+                while n == 0 and ahead < min(count, st) and ok:
+                    ok = yield self.empty[ahead % st], ahead // st - 1
+                    if ok:
+                        self._fetch(ahead)
+                        ahead += 1
+                for i in range(count):
+                    if ok and i >= ahead:
+                        ok = yield self.empty[n % st], n // st - 1
+                        if ok:
+                            self._fetch(n)
+                    if not ok:
+                        break
+                    self._arrive(n)
+                    n += 1
+                issued = max(n, ahead)
+                if not ok:
+                    break
+            if not ok:
+                break
+        for n in range(n, issued):
+            self._arrive(n)
+        n = max(n, issued)
+        for j in range(max(n - st, 0), n):
+            yield self.full[j % st], j // st, "drain"
+
+    def _fetch(self, n):
+        """Announces the bytes of a copy without arriving."""
+        bar = self.full[n % self.STAGES]
+        bar.tx += 1
+        self.mem[n % self.STAGES] = None
+        self.copies.append((bar, n % self.STAGES, n))
+
+    def _arrive(self, n):
+        self.full[n % self.STAGES].arrive()
+
+    def consumer(self, w):
+        n = met = 0
+        ok = True
+        for item, tiles in enumerate(self.items):
+            sums = []
+            for t in range(tiles):
+                st = n % self.STAGES
+                ok = ok and (yield self.full[st], n // self.STAGES)
+                if ok:
+                    assert self.mem[st] == n
+                    yield None
+                    assert self.mem[st] == n
+                    sums.append((w, t))
+                    self.empty[st].arrive()
+                n += 1
+            self.seen.setdefault(item, []).extend(sums)
+            if not ok:
+                self.fail = True
+            self.meet.arrive()
+            yield self.meet, met, "meet"
+            met += 1
+            if ok if self.forget else not self.fail:
+                self.stored[item] = tiles
+                want = sorted((v, t) for v in range(self.WARPS) for t in range(tiles))
+                assert sorted(self.seen[item]) == want, "rows without all of their keys"
             else:
-                assert moves, "a wait for copies or products that were never issued"
-                kind, *what = self.rng.choice(moves)
-                if kind == "role":
-                    self._resume(roles, what[0], True)
-                else:
-                    self.agent(kind, what[0])
-        assert not self.copies and not any(self.queue), "something is in flight behind the last role"
-        return gave_up
-
-    def _resume(self, roles, r, answer):
-        try:
-            roles[r] = r.send(answer)
-        except StopIteration:
-            del roles[r]
+                self.kept.add(item)
+            self.meet.arrive()
+            yield self.meet, met, "meet"
+            met += 1
 
 
 def random_items(rng):
