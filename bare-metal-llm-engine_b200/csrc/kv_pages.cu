@@ -47,6 +47,7 @@ KvView kv_view(const engine_kv_pages_t* kv, int64_t layer) {
   c.vs = kv->v_scale + sc;
   c.table = kv->table;
   c.length = kv->length;
+  c.ref = kv->ref;
   c.n_pages = kv->n_pages;
   c.max_pages = static_cast<int>(kv->max_pages);
   c.n_slots = static_cast<int>(kv->n_slots);
@@ -135,6 +136,15 @@ __device__ int64_t wr_find(const WrParams& p, int64_t item, int* nth) {
   return s_seq;
 }
 
+/// Whether a page with `users` users takes rows: one that others use too (or that is free) is left
+/// as it is (error bit 2).  A write behind an extend that was refused comes to the slot's last
+/// rows, which a fork may have shared.
+__device__ __forceinline__ bool wr_own(const WrParams& p, int users) {
+  if (users == 1) return true;
+  if (threadIdx.x == 0) atomicOr(p.c.err, kErrBadArgument);
+  return false;
+}
+
 /// Largest magnitude of 8 halves, as two packed bit patterns.
 __device__ __forceinline__ uint32_t half8_max(const uint4& x) {
   return __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
@@ -204,6 +214,7 @@ __global__ void __launch_bounds__(kWrThreads) kv_write_kernel(const WrParams p) 
   const int entry = (start >> p.c.shift) + nth;
   const int page = kv_page(p.c, slot, entry);
   if (page < 0) return;
+  const int users = p.c.ref[page];
   const int first = max(start - entry * page_size, 0);  // first new row in the page
   const int rows = min(len - entry * page_size, page_size) - first;
   const int lpr = p.d >> 3;  // threads per row
@@ -223,6 +234,7 @@ __global__ void __launch_bounds__(kWrThreads) kv_write_kernel(const WrParams p) 
   uint4 next[PASSES];
   int tile = blockIdx.y * kWrTiles;
   load(tile, next);
+  if (!wr_own(p, users)) return;  // (looked up beside the rows)
   for (; tile < end; ++tile) {
     const int h = tile >> 1;
     const bool is_v = tile & 1;
@@ -277,6 +289,7 @@ __global__ void __launch_bounds__(kWrThreads) kv_append_kernel(const WrParams p)
   if (wr_rows(p, blockIdx.x, &slot, &r0, &len) == 0) return;
   const int page = kv_page(p.c, slot, (len - 1) >> p.c.shift);
   if (page < 0) return;
+  const int users = p.c.ref[page];
   const int first = (len - 1) & ((1 << p.c.shift) - 1);
   const bool live = tile < 2 * p.c.heads, is_v = tile & 1;
   const int h = live ? tile >> 1 : 0;
@@ -284,6 +297,7 @@ __global__ void __launch_bounds__(kWrThreads) kv_append_kernel(const WrParams p)
   const uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
   float* sp = (is_v ? p.c.vs : p.c.ks) + kv_scale_at(p.c, page, h);
   const float old = live && first > 0 ? *sp : 0.0f;
+  if (!wr_own(p, users)) return;
   uint32_t mx = half8_max(x);
   mx = max(mx & 0xffffu, mx >> 16);
   for (int o = 1; o < lpr; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));

@@ -21,6 +21,7 @@ struct KvView {
   float* vs;
   const int32_t* table;
   int32_t* length;
+  const int32_t* ref;
   int64_t n_pages;
   int max_pages;   // entries of a table row
   int n_slots;

@@ -467,8 +467,10 @@ ENGINE_B200_API int engine_cuda_kv_pages_compact(const engine_kv_pages_t* kv, in
  * codes q become round(q * (old / new)).  A new row's codes are round(x * (1 / scale))
  * (0 for scale 0).  An infinity or NaN cannot be held in 8 bits: the scale
  * becomes NaN, so that attention to that (page, head) answers NaN.
- *   Pages written to must have one user (extend and fork see to that), and a slot
- * occurs once in a call.  k_new, v_new 16-byte aligned, row_pitch a multiple of 8
+ *   Only pages with one user take rows: rows that fall into a page that other
+ * slots use too, or none, are left out with error bit 2.  (Behind an extend that
+ * was refused a slot's last rows are older ones, and forks may share them.)  A
+ * slot occurs once in a call.  k_new, v_new 16-byte aligned, row_pitch a multiple of 8
  * (ENGINE_ERR_UNSUPPORTED otherwise). */
 ENGINE_B200_API int engine_cuda_kv_pages_write(const engine_kv_pages_t* kv, int64_t layer,
                                                const engine_half_t* k_new,

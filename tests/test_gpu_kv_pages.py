@@ -140,6 +140,44 @@ def test_write_leaves_the_rest_alone(pkg, dev):
         assert torch.equal(t[0], b[0]) and torch.equal(t[2], b[2])
 
 
+@pytest.mark.parametrize("dtype", [I8, E4M3])
+def test_write_leaves_shared_pages_alone(pkg, dev, dtype):
+    """Rows of a slot that was forked at a page's end and not extended: the page has two users and
+    stays; the batch's other rows, and the slot's rows in pages of its own, are written."""
+    page, d, hk = 16, 64, 2
+    m, kv = make(pkg, dev, page=page, d=d, hk=hk, dtype=dtype)
+    grow(pkg, m, kv, [0, 1], [2 * page, 7], dev, 1)
+    assert int(pkg.ops.kv_pages_fork(kv, i32([0, 0], dev), i32([3, 4], dev))) == m.fork([0, 0], [3, 4]) == 0
+    pkg.ops.kv_pages_extend(kv, i32([1], dev), i32([1], dev))
+    m.extend([1], [1])
+    rows = 5 * torch.randn(4, hk * d, generator=torch.Generator().manual_seed(2)).half()
+    on = rows.to(dev)
+    for slots in ([3, 1], [4, 1], [0, 1]):  # one row each; slot 1's row is rewritten
+        pkg.ops.kv_pages_write(kv, 0, on[:2], on[2:], i32(slots, dev))
+        assert pkg.device_status() == 2
+    m.write(0, rows[1:2], rows[3:4], [1], [0, 1])
+    m.write(0, rows[1:2], rows[3:4], [1], [0, 1])
+    m.write(0, rows[1:2], rows[3:4], [1], [0, 1])
+    m.same_books(kv)
+    m.same_data(kv)
+    # ragged: five rows of slot 3, of which three fall into the shared page; slot 1 as it is
+    assert int(pkg.ops.kv_pages_extend(kv, i32([3], dev), i32([2], dev))) == m.extend([3], [2]) == 0
+    rows = 5 * torch.randn(6, hk * d, generator=torch.Generator().manual_seed(3)).half()
+    on = rows.to(dev)
+    pkg.ops.kv_pages_write(kv, 0, on, on, i32([3, 1], dev), i32([0, 5, 6], dev))
+    assert pkg.device_status() == 2
+    m.write(0, rows[3:], rows[3:], [3, 1], [0, 2, 3])
+    m.same_books(kv)
+    m.same_data(kv)
+    # with its own pages alone, nothing is left out
+    pkg.ops.kv_pages_free(kv, i32([0, 4], dev))
+    m.free([0, 4])
+    pkg.ops.kv_pages_write(kv, 0, on, on, i32([3, 1], dev), i32([0, 5, 6], dev))
+    m.write(0, rows, rows, [3, 1], [0, 5, 6])
+    assert pkg.device_status() == 0
+    m.same_data(kv)
+
+
 # ------------------------------------------------------------ bookkeeping
 
 
