@@ -467,7 +467,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t tS = tmem + (static_cast<uint32_t>(r0) << 16) + side * 128;
     const uint32_t tO = tmem + (static_cast<uint32_t>(r0) << 16) + Cfg::kColO + side * D;
     int n = 0, own = 0, both = 0;  // tiles, those of this side, and those with a side B
-    int idle = 0;                  // tiles of items without this side since its last one
     bool ok = true;
     // Token within the side's, or far past any, and head within the group of the thread's rows.
     int q_tok[2], q_head[2];
@@ -480,10 +479,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int x = lo; x < hi && ok && it.t0 < it.t1;) {
       if (side == 1 && !it.two) {
         n += it.t1 - it.t0;
-        idle += it.t1 - it.t0;
         x = tc_end(it);
         if (x < hi) tc_next(p, it, x, hi);
         continue;
+      }
+      // Side B's first S of an item comes behind the tiles of those without rows for it (n - own so
+      // far), each of which may take what a wait may.
+      if (n != own) {
+        ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->s_full[side], own & 1, limit * (min(n - own, 4095) + 1), c.err));
+        if (!ok) break;
       }
       const int left = it.n_tok - (it.qb * 2 + side) * p.tq;  // tokens of the sequence from the side's first on
       int lim[2];
@@ -494,10 +498,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int t = it.t0; t < it.t1; ++t, ++n, ++own, both += it.two ? 1 : 0) {
         const float4* con = s_const + (n & 3) * 8;
         const int key = t * kTcKeys + 2 * t4;
-        // The other side's tiles in between take a tile's time each.
-        ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->s_full[side], own & 1, limit * (min(idle, 4095) + 1), c.err));
+        ok = __all_sync(0xffffffffu, mbar_wait_sleepy(&bar->s_full[side], own & 1, limit, c.err));
         if (!ok) break;
-        idle = 0;
         tc_fence_after();
         const bool clean =
             __all_sync(0xffffffffu, (t + 1) * kTcKeys <= min(lim[0], lim[1]) && con[0].w == 2.0f);
