@@ -100,6 +100,7 @@ EXPORTS: dict[str, list] = {
     "engine_cuda_kv_pages_free": [_p, _p, _i64, _p],
     "engine_cuda_kv_pages_compact": [_p, _p, _p],
     "engine_cuda_kv_pages_write": [_p, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _p],
+    "engine_cuda_kv_pages_write_if": [_p, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _p, _p],
     "engine_cuda_attention_paged_decode": [_p, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _f, _p],
     "engine_cuda_attention_paged_prefill": [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64,
                                             _f, ctypes.c_int, _p],

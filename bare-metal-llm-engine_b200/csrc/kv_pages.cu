@@ -77,7 +77,8 @@ struct WrParams {
   const int32_t* slots;
   const int32_t* cu;
   int64_t n_seq, n_tokens;
-  int d;  // head_dim
+  const int32_t* status;  // null, or nothing is written unless *status is 0
+  int d;                  // head_dim
 };
 
 /// New rows of sequence b: [r0, r0 + n), positions [len - n, len).
@@ -201,6 +202,7 @@ template <int PASSES, bool E4M3>
 __global__ void __launch_bounds__(kWrThreads) kv_write_kernel(const WrParams p) {
   pdl_trigger();
   pdl_wait();
+  if (p.status != nullptr && *p.status != 0) return;
   __shared__ uint32_t s_max[2][kWrThreads / 32];
   int nth = 0;
   const int64_t b = wr_find(p, blockIdx.x, &nth);
@@ -281,6 +283,7 @@ template <bool E4M3>
 __global__ void __launch_bounds__(kWrThreads) kv_append_kernel(const WrParams p) {
   pdl_trigger();
   pdl_wait();
+  if (p.status != nullptr && *p.status != 0) return;
   const int lpr = p.d >> 3;
   const int tile = static_cast<int>(blockIdx.y) * (kWrThreads / lpr) + threadIdx.x / lpr;
   const int tc = threadIdx.x % lpr;
@@ -735,6 +738,15 @@ int engine_cuda_kv_pages_write(const engine_kv_pages_t* kv, int64_t layer,
                                const engine_half_t* k_new, const engine_half_t* v_new,
                                int64_t row_pitch, const int32_t* slots, const int32_t* cu_new,
                                int64_t n_seq, int64_t n_tokens, engine_stream_t stream) {
+  return engine_cuda_kv_pages_write_if(kv, layer, k_new, v_new, row_pitch, slots, cu_new, n_seq, n_tokens,
+                                       nullptr, stream);
+}
+
+int engine_cuda_kv_pages_write_if(const engine_kv_pages_t* kv, int64_t layer,
+                                  const engine_half_t* k_new, const engine_half_t* v_new,
+                                  int64_t row_pitch, const int32_t* slots, const int32_t* cu_new,
+                                  int64_t n_seq, int64_t n_tokens, const int32_t* status,
+                                  engine_stream_t stream) {
   B200_ENTRY_BEGIN
   if (const int rc = kv_pages_check(kv, layer, "kv_pages_write")) return rc;
   B200_REQUIRE(layer >= 0, "kv_pages_write: layer out of range");
@@ -768,6 +780,7 @@ int engine_cuda_kv_pages_write(const engine_kv_pages_t* kv, int64_t layer,
   p.cu = cu_new;
   p.n_seq = n_seq;
   p.n_tokens = n_tokens;
+  p.status = status;
   p.d = static_cast<int>(kv->head_dim);
   const bool e4m3 = kv->type == ENGINE_KV_E4M3;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

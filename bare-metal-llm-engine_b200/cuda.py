@@ -229,9 +229,10 @@ def kv_pages_compact(kv, remap=0, stream=0):
     _check(lib().engine_cuda_kv_pages_compact(_kv(kv), remap, _s(stream)))
 
 
-def kv_pages_write(kv, layer, k_new, v_new, row_pitch, slots, cu_new, n_seq, n_tokens, stream=0):
-    _check(lib().engine_cuda_kv_pages_write(_kv(kv), layer, k_new, v_new, row_pitch, slots, cu_new,
-                                            n_seq, n_tokens, _s(stream)))
+def kv_pages_write(kv, layer, k_new, v_new, row_pitch, slots, cu_new, n_seq, n_tokens, stream=0,
+                   status=0):
+    _check(lib().engine_cuda_kv_pages_write_if(_kv(kv), layer, k_new, v_new, row_pitch, slots, cu_new,
+                                               n_seq, n_tokens, status, _s(stream)))
 
 
 def attention_paged_decode(kv, layer, q, q_pitch, slots, out, out_lse, n_seq, n_heads, scale,

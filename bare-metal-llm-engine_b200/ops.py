@@ -392,11 +392,13 @@ def _kv_f16(kv, t, name):
         raise ValueError(f"{name} must be on the cache's device")
 
 
-def kv_pages_write(kv, layer: int, k_rows, v_rows, slots=None, cu_new=None):
+def kv_pages_write(kv, layer: int, k_rows, v_rows, slots=None, cu_new=None, status=None):
     """Stores K / V rows [n_tokens, H_kv * d] (FP16, rows may be strided views, e.g. the
     columns of a fused Q/K/V projection) as the LAST positions of the slots: rows
     [cu_new[i], cu_new[i+1]) of slot slots[i], or one row each where cu_new is None.
-    Call kv_pages_extend first: it counts them."""
+    Call kv_pages_extend first: it counts them.  With its `status` given, nothing is written
+    unless that is 0 (behind an extend that was refused, the last positions are those of earlier
+    rows); a step that does not read it on the host, a captured one, passes it on."""
     st = _kv_stream(kv)
     _kv_f16(kv, k_rows, "k_rows")
     _kv_f16(kv, v_rows, "v_rows")
@@ -409,9 +411,12 @@ def kv_pages_write(kv, layer: int, k_rows, v_rows, slots=None, cu_new=None):
     n_seq, cu = n_tokens, 0
     if cu_new is not None:
         n_seq, cu = cu_new.numel() - 1, _kv_i32(kv, cu_new, "cu_new")
+    if status is not None and status.numel() != 1:
+        raise ValueError("status must be the one word of kv_pages_extend")
     _c.kv_pages_write(kv.handle, layer, k_rows.data_ptr(), v_rows.data_ptr(),
                       stride[0] if n_tokens > 1 else max(stride[0], kv.width),
-                      _kv_slots(kv, slots, n_seq), cu, n_seq, n_tokens, st)
+                      _kv_slots(kv, slots, n_seq), cu, n_seq, n_tokens, st,
+                      0 if status is None else _kv_i32(kv, status, "status"))
 
 
 def _paged_q(kv, q, out):

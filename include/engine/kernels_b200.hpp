@@ -254,14 +254,15 @@ inline void kv_pages_compact(const KvPages& kv, std::int32_t* remap = nullptr,
                              cudaStream_t stream = 0) {
   b200_detail::check(engine_cuda_kv_pages_compact(&kv, remap, stream));
 }
-// cu_new null: one row per sequence, n_tokens = n_seq.
+// cu_new null: one row per sequence, n_tokens = n_seq.  status: the device word of the
+// extend before; nothing is written unless it is 0.
 inline void kv_pages_write(const KvPages& kv, std::int64_t layer, const __half* k_new,
                            const __half* v_new, std::int64_t row_pitch, const std::int32_t* slots,
                            const std::int32_t* cu_new, std::int64_t n_seq, std::int64_t n_tokens,
-                           cudaStream_t stream = 0) {
-  b200_detail::check(engine_cuda_kv_pages_write(&kv, layer, b200_detail::h(k_new),
-                                                b200_detail::h(v_new), row_pitch, slots, cu_new,
-                                                n_seq, n_tokens, stream));
+                           cudaStream_t stream = 0, const std::int32_t* status = nullptr) {
+  b200_detail::check(engine_cuda_kv_pages_write_if(&kv, layer, b200_detail::h(k_new),
+                                                   b200_detail::h(v_new), row_pitch, slots, cu_new,
+                                                   n_seq, n_tokens, status, stream));
 }
 inline void attention_paged_decode(const KvPages& kv, std::int64_t layer, const __half* q,
                                    std::int64_t q_pitch, const std::int32_t* slots, __half* out,

@@ -479,6 +479,17 @@ ENGINE_B200_API int engine_cuda_kv_pages_write(const engine_kv_pages_t* kv, int6
                                                int64_t n_seq, int64_t n_tokens,
                                                engine_stream_t stream);
 
+/* The same where *status (device; the word of the extend before, may be null) is
+ * 0, and nothing otherwise: a slot's last positions are then those of earlier
+ * rows.  For steps that do not read the word on the host before the write, a
+ * captured one for instance. */
+ENGINE_B200_API int engine_cuda_kv_pages_write_if(const engine_kv_pages_t* kv, int64_t layer,
+                                                  const engine_half_t* k_new,
+                                                  const engine_half_t* v_new, int64_t row_pitch,
+                                                  const int32_t* slots, const int32_t* cu_new,
+                                                  int64_t n_seq, int64_t n_tokens,
+                                                  const int32_t* status, engine_stream_t stream);
+
 /* attention_decode (kernels.hpp:191) over the paged cache for a ragged batch:
  * out[i][h] = softmax(scale q[i][h] K^T) V over the length[slots[i]] positions of
  * its slot.  q row i at i * q_pitch elements, [n_heads][head_dim]; out

@@ -600,6 +600,50 @@ def test_captured_decode_step(pkg, dev):
     m.same_data(kv)
 
 
+@pytest.mark.parametrize("ragged", [False, True])
+def test_a_step_whose_extend_is_refused_leaves_the_cache(pkg, dev, ragged):
+    """extend, write and decode captured once, the write with the extend's status: a replay that
+    lacks pages changes nothing, and the next one after a free goes on as if it had not been."""
+    heads, hk, d, page = 8, 2, 64, 16
+    m, kv = make(pkg, dev, layers=2, hk=hk, d=d, page=page, slots=5, n_pages=7, max_pages=4)
+    grow(pkg, m, kv, [0, 1, 4], [30, 32, 17], dev, 1)  # 2 + 2 + 2 pages; slot 1 is at a page's end
+    assert int(pkg.ops.kv_pages_fork(kv, i32([1], dev), i32([3], dev))) == m.fork([1], [3]) == 0
+    slots, n = i32([0, 1, 3], dev), i32([1, 1, 1], dev)
+    cu = i32([0, 1, 2, 3], dev) if ragged else None
+    rows = torch.zeros(3, 2, hk * d, device=dev, dtype=torch.float16)
+    q = torch.randn(3, heads, d, generator=torch.Generator().manual_seed(2)).half().to(dev)
+
+    def step():
+        st = pkg.ops.kv_pages_extend(kv, slots, n)
+        for layer in range(2):
+            pkg.ops.kv_pages_write(kv, layer, rows[:, 0], rows[:, 1], slots, cu, status=st)
+        return st, pkg.ops.attention_paged_decode(kv, 1, q, slots)
+
+    pkg.ops.attention_paged_decode(kv, 0, q, slots)  # warm
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        st, out = step()
+    for i in range(3):  # two pages are wanted, one is free; the third time two more are
+        new = torch.randn(3, 2, hk * d, generator=torch.Generator().manual_seed(10 + i)).half()
+        rows.copy_(9 * new)
+        if i == 2:
+            pkg.ops.kv_pages_free(kv, i32([4], dev))
+            m.free([4])
+        graph.replay()
+        want = m.extend([0, 1, 3], [1, 1, 1])
+        assert int(st) == want == (0 if i == 2 else 1)
+        if want == 0:
+            for layer in range(2):
+                m.write(layer, 9 * new[:, 0], 9 * new[:, 1], [0, 1, 3], [0, 1, 2, 3])
+        m.same_books(kv)
+        m.same_data(kv)
+    assert pkg.device_status() == 0
+    ref.check_attention(kv, 1, q, out, [0, 1, 3], [0, 1, 2, 3], d ** -0.5)
+    with pytest.raises(ValueError, match="status must be the one word"):
+        pkg.ops.kv_pages_write(kv, 0, rows[:, 0], rows[:, 1], slots, cu, status=n)
+
+
 def test_two_attentions_at_once(pkg, dev):
     """Calls on two streams that run together do not share anything."""
     m, kv = make(pkg, dev, hk=2, d=128, page=64, slots=3, n_pages=150, max_pages=70)

@@ -206,3 +206,19 @@ def test_restatement_rounds_to_the_nearest(dtype):
     assert m.fork([1], [0]) == 0 and m.ref == [2, 1, 1, 0, 0, 0, 0, 0]
     m.free([1])
     assert m.compact() == [0, -1, 1, -1, -1, -1, -1, -1] and m.rows[0] == [0, 1]
+
+
+def test_write_with_a_status_checks_its_arguments(pkg):
+    """The call with the word of an extend refuses what the call without it does."""
+    w, kv = pkg.lib().engine_cuda_kv_pages_write_if, desc(pkg)
+    import ctypes
+
+    def bad(*args, code=1, substr=""):
+        assert w(ctypes.addressof(kv), *args) == code
+        assert substr in pkg.lib().engine_last_error().decode()
+
+    bad(2, P, P, 1024, P, P, 1, 1, P, 0, substr="layer out of range")
+    bad(0, P, P, 1023, P, P, 1, 1, P, 0, substr="row_pitch <")
+    bad(0, 0, P, 1024, P, P, 1, 1, P, 0, substr="k_new/v_new is null")
+    bad(0, P, P, 1028, P, P, 1, 1, P, 0, code=3, substr="multiple of 8")
+    assert w(ctypes.addressof(kv), 0, 0, 0, 1024, 0, 0, 0, 0, P, 0) == 0  # nothing to write
