@@ -405,16 +405,16 @@ def kv_pages_write(kv, layer: int, k_rows, v_rows, slots=None, cu_new=None, stat
     shape, stride = k_rows.shape, k_rows.stride()
     if len(shape) != 2 or shape[1] != kv.width:
         raise ValueError("k_rows must be [n_tokens, H_kv * d]")
-    if v_rows.shape != shape or v_rows.stride() != stride or stride[1] != 1:
-        raise ValueError("k_rows / v_rows: rows must be contiguous, as many, and share one pitch")
     n_tokens = shape[0]
+    if v_rows.shape != shape or stride[1] != 1 or v_rows.stride(1) != 1 or (n_tokens > 1 and v_rows.stride(0) != stride[0]):
+        raise ValueError("k_rows / v_rows: rows must be contiguous, as many, and share one pitch")
     n_seq, cu = n_tokens, 0
     if cu_new is not None:
         n_seq, cu = cu_new.numel() - 1, _kv_i32(kv, cu_new, "cu_new")
     if status is not None and status.numel() != 1:
         raise ValueError("status must be the one word of kv_pages_extend")
     _c.kv_pages_write(kv.handle, layer, k_rows.data_ptr(), v_rows.data_ptr(),
-                      stride[0] if n_tokens > 1 else max(stride[0], kv.width),
+                      stride[0] if n_tokens > 1 else kv.width,
                       _kv_slots(kv, slots, n_seq), cu, n_seq, n_tokens, st,
                       0 if status is None else _kv_i32(kv, status, "status"))
 
@@ -434,7 +434,7 @@ def _paged_q(kv, q, out):
         _req(out, torch.float16, "out")
         if out.shape != shape or out.get_device() != kv.device_index:
             raise ValueError("out must have q's shape and device")
-    return n, H, (stride[0] if n > 1 else max(stride[0], H * d)), out
+    return n, H, (stride[0] if n > 1 else H * d), out
 
 
 def attention_paged_decode(kv, layer: int, q, slots=None, scale=None, out=None,

@@ -178,6 +178,24 @@ def test_write_leaves_shared_pages_alone(pkg, dev, dtype):
     m.same_data(kv)
 
 
+def test_one_row_has_any_pitch(pkg, dev):
+    """A single row's pitch is no part of it: views whose rows are 8 n + 3 elements apart, of K and
+    V in tensors of different widths."""
+    d, hk, heads = 64, 2, 8
+    m, kv = make(pkg, dev, d=d, hk=hk)
+    grow(pkg, m, kv, [2], [20], dev, 1)
+    assert int(pkg.ops.kv_pages_extend(kv, i32([2], dev), i32([1], dev))) == m.extend([2], [1]) == 0
+    k, v, q = (torch.randn(1, n, generator=torch.Generator().manual_seed(n)).half() for n in (395, 261, 1027))
+    on = [t.to(dev) for t in (k, v, q)]
+    pkg.ops.kv_pages_write(kv, 0, on[0][:, 128:256], on[1][:, :128], i32([2], dev))
+    m.write(0, k[:, 128:256], v[:, :128], [2], [0, 1])
+    m.same_data(kv)
+    one = on[2][:, 8:8 + heads * d].view(1, heads, d)
+    got = pkg.ops.attention_paged_decode(kv, 0, one, i32([2], dev))
+    ref.check_attention(kv, 0, one, got, [2], [0, 1], d ** -0.5)
+    assert torch.equal(got, pkg.ops.attention_paged_prefill(kv, 0, one, i32([2], dev), i32([0, 1], dev)))
+
+
 # ------------------------------------------------------------ bookkeeping
 
 
