@@ -728,14 +728,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
   const int parts = static_cast<int>(static_cast<unsigned>(cut.z) >> 16);
   const int part0 = 2 * cut.w;
   auto slot = [&](int i) { return static_cast<int64_t>(part0 + (i == 0 ? 1 : 2 * i)) * kPgRows + row; };
-  float m = -INFINITY;
-  bool all = true;
+  float m = -INFINITY, least = 0.0f;
   for (int i = lane; i < parts; i += 32) {
     const float2 ml = p.ws_ml[slot(i)];
     m = fmaxf(m, ml.x);
-    all &= ml.y != kNoPart;
+    least = fminf(least, ml.y);
   }
-  if (!__all_sync(0xffffffffu, all)) return;  // (every warp of a row looks at all parts)
+  if (__any_sync(0xffffffffu, least == kNoPart)) return;  // (every warp of a row looks at all parts)
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
   float l = 0.0f, o[E] = {};

@@ -827,15 +827,14 @@ __global__ void __launch_bounds__(2 * D) attn_paged_tc_join_kernel(const TcParam
   auto part = [&](int i) {
     return (static_cast<int64_t>(blockIdx.x) * 2 + (i == 0 ? 1 : 2 * i)) * kTcRows + flat;
   };
-  float m = -INFINITY;
-  bool all = true;
+  float m = -INFINITY, least = 0.0f;
 #pragma unroll 4
   for (int i = 0; i < parts; ++i) {
     const float2 ml = p.a.ws_ml[part(i)];
     m = fmaxf(m, ml.x);
-    all &= ml.y != kNoPart;
+    least = fminf(least, ml.y);
   }
-  if (!all) return;
+  if (least == kNoPart) return;
   float l = 0.0f;
   float4 o = make_float4(0, 0, 0, 0);
 #pragma unroll 2
