@@ -7,7 +7,15 @@
 // m the running maximum of x_j + log2 vs_j.  Keeping the page's scale of V inside
 // the weight leaves the products to the codes alone, and the weight is scaled by
 // what it contributes.  A page whose values are all zero has scale 0: it counts
-// with vs = 1 (its codes are zeros).
+// with vs = kNoScale = 2^-33 (its codes are zeros).  That is below every scale that a
+// write gives, so its weights never set the m that the others' are rounded against
+// (with 1, values of 1e-3 beside a dominant key in such a page lost 20 times the bound).
+//
+// w goes into the second product as FP16 (off by 2^-11 of itself at most, below 2^-14 by
+// half a step of 2^-24): the tensor cores take 16 bits beside the codes, and the codes
+// are exact there.  m, l and the sums of both products stay in FP32, l from the weights
+// before that rounding.  Outputs are 2.3e-4 to 2.9e-4 (relative, RMS) from 64 bits, of which
+// their own FP16 rounding is 2.0e-4.
 //
 // Few query rows per KV head (decode, and the verification of a few tokens): the
 // keys and values are the traffic, 2 bytes for 4 * rows FLOP, so what counts is
@@ -30,12 +38,18 @@
 // are consecutive bytes: D / 4 of two keys' rows for S^T, D / 8 of four keys' rows for
 // O^T; P passes from one layout to the other by two 8 x 8 transpositions.
 //   Measured (B200, 32 / 8 heads of 128, calls back to back): 131072 keys of one sequence
-// 54 us (269 MB, 0.75 of the measured copy rate), 48 sequences of 200-16384 keys 74 us (372
+// 55 us (269 MB, 0.75 of the measured copy rate), 48 sequences of 200-16384 keys 74 us (372
 // MB, 0.77), 64 x 4000 keys 94 us (0.85).  Within the kernel the tiles arrive at about 7 TB/s;
 // the rest is the 5 us until the first tile is there (lengths, table, scales and codes, each
 // looked up with the last), the spread of the shares' ends and the join (4 us).  With q as A
 // and the int8 offset taken off every code the first was 66 us where it is 54 to 55.  Eight
-// consumer warps a CTA, two CTAs: 96 registers, spills, 83.
+// consumer warps a CTA, two CTAs: 96 registers, spills, 83.  Items of 16 rows with d = 128
+// spill too (int8 124 bytes of stores, e4m3 32, by -Xptxas -v): 1.9 % of the instructions of 16
+// x 4 rows on 4000 keys.
+//
+//   Every wait is bounded (ENGINE_WAIT_TIMEOUT_MS).  Behind one that ran out the CTA stores no
+// more rows and marks its parts, so that the join leaves theirs alone; copies in flight are waited
+// for before it ends.
 
 #include <algorithm>
 #include <atomic>
@@ -57,12 +71,15 @@ constexpr float kPgRescale = 8.0f;
 /// front of the item's tiles in which nothing is done.  48 sequences of 200-16384 keys: 75 us
 /// with 2, 72 with 4, 74 with 8.
 constexpr int kPgItemCost = 4;
-/// Query rows of a sequence and KV head (the average: the host knows no more) from which
+/// Query rows of a sequence and KV head (the average: the host knows no more, and a call that
+/// mixes prompts with single rows pays for it: 512 rows on 8704 keys with 63 or 200 single rows on
+/// 4000 keys take 368 and 765 us, in two calls 198 and 392) from which
 /// attention_paged_tc takes the call: what needs a third group of 16 here.  One sequence of
 /// 4000 keys: 32 rows 23 us either way, 48 rows 23 us there and 24 here, 64 rows 23 and 25;
 /// sixteen of them: 16 rows 83 and 52, 32 rows 81 and 77, 48 rows 82 and 103.
 constexpr int64_t kManyRows = 33;
-/// Slots of at most so many tiles have a CTA to an item: no workspace, no join.  1000 keys: one
+/// Slots of at most so many tiles (by the table's width: the host knows no lengths) have a CTA to an
+/// item: no workspace, no join.  1000 keys: one
 /// sequence 13 us and 16 split, 8 sequences 14 and 16, 256 sequences 102 and 103; at 2000 keys
 /// (32 tiles) it would be 21 and 16, 26 and 20, 176 and 179.
 constexpr int64_t kWholeTiles = 16;

@@ -22,18 +22,21 @@
 // and B.  Within a side, S -> softmax -> P V is a chain; the two sides' chains interleave
 // on the tensor cores and the exponential units.
 //
-//   Measured (B200, 32 / 8 heads of 128, calls back to back): 512 rows on 8704 keys 94 us (753
-// TFLOP/s, 0.45 of the measured burst), a 4096-token prompt 172 us.  A side's chain bounds
+//   Measured (B200, 32 / 8 heads of 128, calls back to back): 512 rows on 8704 keys 95 us (745
+// TFLOP/s, 0.45 of the measured burst), a 4096-token prompt 180 us.  A side's chain bounds
 // it: of about 4100 cycles a tile, 700 are the maxima, 1700 the weights (exponentials 512 of
 // each half's 850), 1600 from the last weight to the next tile's S.  Steps: one thread a row
 // with S in 128 registers 117 us; four threads a row 135; one MMA thread for both sides, whose
 // issue was the bound, to a warp a side and descriptors that differ by constants 119; the
 // sides' turns and the maxima before them 93; the first half's scores kept 92 to 94.  Without
-// the turns 103 (four prompts of 700-5000 tokens 406, 378 with them).
+// the turns 102; four prompts of 700-5000 tokens 405 without, 390 to 404 with them.  The 80
+// registers at launch spill (460 to 596 bytes of stores, by -Xptxas -v): 1.4 % of the chunk's
+// instructions.
 //
 // Every wait is bounded (ENGINE_WAIT_TIMEOUT_MS): on expiry the warp sets the device
 // error word, its role ends, the others' waits run out too, and all meet at the
 // teardown, where copies and MMAs in flight are waited for (by a limit of their own).
+// Rows whose products are not complete are not stored, nor joined.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -255,8 +258,8 @@ __device__ __forceinline__ void tc_half_max(const uint32_t (&v)[32], const float
   }
 }
 
-/// The weights against the references m, as FP16 pairs in the order of
-/// tmem_st_16x128b_x8; adds the thread's w / vs to l.
+/// The weights against the references m, as FP16 pairs (see attention_paged.cu) in the order of
+/// tmem_st_16x128b_x8; adds the thread's w / vs to l, before that rounding.
 template <int KG>
 __device__ __forceinline__ void tc_half_weights(const uint32_t (&v)[32], const float4* con, bool clean,
                                                 const float (&m)[2], float (&l)[2], uint32_t (&pk)[16]) {

@@ -455,7 +455,8 @@ def attention_paged_prefill(kv, layer: int, q, slots, cu_q, scale=None, out=None
     """out [T, H, d] of the query rows [cu_q[i], cu_q[i+1]) of q [T, H, d], the LAST
     positions of slot slots[i] (None: slot i), over the slot's positions up to their
     own (all of them unless is_causal).  Rows past cu_q[-1] are left as they were in
-    `out`.  With want_lse also lse [T, H] (FP32)."""
+    `out`.  With want_lse also lse [T, H] (FP32).  Prompts and single rows are faster in two
+    calls: the kernel is chosen by the average number of rows."""
     st = _kv_stream(kv)
     T, H, pitch, o = _paged_q(kv, q, out)
     n_seq, cu = cu_q.numel() - 1, _kv_i32(kv, cu_q, "cu_q")

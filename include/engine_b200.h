@@ -35,8 +35,9 @@
  *     kernels with more than one; up to 8 tcgen05 splits merge inside a
  *     thread-block cluster and need none),
  *     engine_cuda_attention_paged_decode / _prefill (the parts of sequences that
- *     are split over CTAs: at most 8 MB, 39 MB with more than 32 query rows per
- *     sequence and KV head; none for slots of at most 1024 positions) and
+ *     are split over CTAs: at most 8 MB, and none where max_pages * page_size is at
+ *     most 1024; at most 40 MB, whatever the table's width, for prefills of 33 query
+ *     rows and more per sequence and KV head, on the average) and
  *     engine_cuda_kv_pages_fork / _compact (a few words per slot or page);
  *   - once per (device, stream), on the first call that needs it, never during
  *     a stream capture: the stream-K workspace of the large 16-bit GEMMs
@@ -508,7 +509,9 @@ ENGINE_B200_API int engine_cuda_attention_paged_decode(const engine_kv_pages_t* 
  * (written before the call); when causal, each sees the positions up to its own,
  * otherwise all of the slot's.  Rows that see nothing get zeros and -inf; the
  * rows from cu_q[n_seq] to n_tokens are left as they were.  q, out, out_lse as
- * for attention_paged_decode, with n_tokens rows. */
+ * for attention_paged_decode, with n_tokens rows.
+ *   One kernel serves the whole call, chosen by the average number of rows per
+ * sequence: prompts (or chunks of them) and single rows are faster in two calls. */
 ENGINE_B200_API int engine_cuda_attention_paged_prefill(const engine_kv_pages_t* kv, int64_t layer,
                                                         const engine_half_t* q, int64_t q_pitch,
                                                         const int32_t* slots, const int32_t* cu_q,
