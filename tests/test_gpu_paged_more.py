@@ -143,3 +143,53 @@ def test_the_cache_against_the_rows_that_were_written(pkg, dev, dtype, one_by_on
         bound = np.expm1(2 * e) * (p @ np.abs(v)) + np.exp(2 * e) * (p @ off[1, :, h // 4].numpy()) + own[0, h]
         assert (np.abs(out[h] - p @ v) <= bound).all(), (h, (np.abs(out[h] - p @ v) / bound).max())
     assert pkg.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [I8, E4M3])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 16), (64, 128)])
+def test_the_smallest_pool(pkg, dev, dtype, d, page):
+    """One page, one KV head, one slot: both attention kernels, with fewer rows in the pool than a
+    tile has, and a fork and an extend that it cannot meet."""
+    kv = filled(pkg, dev, [page - 3], hk=1, d=d, page=page, max_pages=1, dtype=dtype, spare=1)
+    kv.ref[1:] = 1  # (`filled` leaves a page free)
+    for rows in (1, 3, 40):
+        q = torch.randn(rows, 2, d, generator=torch.Generator().manual_seed(rows)).half().to(dev)
+        out, lse = pkg.ops.attention_paged_prefill(kv, 0, q, i32([0], dev), i32([0, rows], dev), want_lse=True)
+        ref.check_attention(kv, 0, q, out, [0], [0, rows], d ** -0.5, lse=lse)
+    assert int(pkg.ops.kv_pages_fork(kv, i32([0], dev), i32([1], dev))) == 1
+    assert int(pkg.ops.kv_pages_extend(kv, i32([0, 1], dev), i32([3, 1], dev))) == 1
+    assert int(pkg.ops.kv_pages_extend(kv, i32([0], dev), i32([3], dev))) == 0
+    assert kv.length.tolist() == [page, 0] and kv.table.tolist() == [[0], [-1]]
+    assert pkg.device_status() == 0
+
+
+def test_host_threads_at_once(pkg, dev):
+    """Eight host threads, each with a stream and a cache of its own, step at once."""
+    import threading
+
+    wrong = []
+
+    def work(i):
+        try:
+            torch.cuda.set_device(dev)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                lens = [40 + 300 * i, 1 + i]
+                kv = filled(pkg, dev, lens, hk=2, d=64 if i % 2 else 128, page=32, max_pages=80, dtype=I8 if i % 3 else E4M3)
+                d = kv.head_dim
+                q = torch.randn(30, 8, d, generator=torch.Generator().manual_seed(i)).half().to(dev)
+                for _ in range(5):
+                    one = pkg.ops.attention_paged_decode(kv, 0, q[:2])
+                    many = pkg.ops.attention_paged_prefill(kv, 0, q, None, i32([0, 29, 30], dev))
+                torch.cuda.current_stream().synchronize()
+                ref.check_attention(kv, 0, q[:2], one, [0, 1], [0, 1, 2], d ** -0.5)
+                ref.check_attention(kv, 0, q, many, [0, 1], [0, 29, 30], d ** -0.5)
+        except BaseException as e:  # noqa: BLE001 (told to the main thread)
+            wrong.append((i, e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
+    assert pkg.device_status() == 0
