@@ -53,14 +53,14 @@ __device__ __forceinline__ int kv_slot(const KvView& c, const int32_t* slots, in
   return static_cast<int>(s);
 }
 
-/// Length of a slot (0 for slot -1), held to what its table row can address.
+/// Length of a slot: 0 for slot -1, and (with error bit 2) for one that its table row cannot address.
 __device__ __forceinline__ int kv_length(const KvView& c, int slot) {
   if (slot < 0) return 0;
   const int n = c.length[slot];
   const int64_t cap = static_cast<int64_t>(c.max_pages) << c.shift;
   if (n < 0 || n > cap) {
     atomicOr(c.err, kErrBadArgument);
-    return n < 0 ? 0 : static_cast<int>(cap);
+    return 0;
   }
   return n;
 }

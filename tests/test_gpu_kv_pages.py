@@ -490,6 +490,35 @@ def test_bad_entries_are_left_out(pkg, dev):
     assert torch.equal(kv.k, before)
 
 
+@pytest.mark.parametrize("length", [65, 2 ** 31 - 1, -1, -2 ** 31])
+def test_lengths_that_a_row_cannot_hold_are_left_out(pkg, dev, length):
+    """A slot whose length is beyond its table row, every entry of which is in use: its rows are not
+    written and its attention is that of an empty slot; the batch's other slot is as it was."""
+    m, kv = make(pkg, dev, page=16, d=64, hk=2, slots=3, max_pages=4)
+    grow(pkg, m, kv, [0, 1], [64, 20], dev, 1)
+    q = torch.randn(60, 8, 64, generator=torch.Generator().manual_seed(1)).half().to(dev)
+    want = pkg.ops.attention_paged_decode(kv, 0, q[:2])[1]
+    rows = 5 * torch.randn(41, 128, generator=torch.Generator().manual_seed(2)).half()
+    on = rows.to(dev)
+    kv.length[0] = length
+    pkg.ops.kv_pages_write(kv, 0, on[:1], on[:1], i32([0], dev))
+    assert pkg.device_status() == 2
+    pkg.ops.kv_pages_write(kv, 0, on, on, i32([0, 1], dev), i32([0, 40, 41], dev))
+    assert pkg.device_status() == 2
+    out, lse = pkg.ops.attention_paged_decode(kv, 0, q[:2], want_lse=True)
+    assert pkg.device_status() == 2
+    assert out[0].eq(0).all() and lse[0].isneginf().all()
+    for r in (3, 50):  # both kernels
+        pre, lse = pkg.ops.attention_paged_prefill(kv, 0, q[:r + 1], None, i32([0, r, r + 1], dev), want_lse=True)
+        assert pkg.device_status() == 2
+        assert pre[:r].eq(0).all() and lse[:r].isneginf().all() and pre[r].isfinite().all()
+    kv.length[0] = 64
+    assert not torch.equal(out[1], want)  # its last row is another one now
+    m.write(0, rows[40:], rows[40:], [1], [0, 1])
+    m.same_books(kv)
+    m.same_data(kv)
+
+
 @pytest.mark.parametrize("n_tokens", [4095, 16384])
 def test_rows_that_overlap_without_end(pkg, dev, n_tokens):
     """Row counts that go back and forth, so that 512 sequences have all of the rows: more work
